@@ -409,6 +409,9 @@ class RLConfig(BaseConfig):
     clip_eps: float = opt(0.2, "PPO clip epsilon")
     kl_beta: float = opt(0.04, "KL penalty to the frozen reference policy")
     kv_block_size: int = opt(16, "tokens per KV-cache page")
+    kv_cache_bits: int = opt(16, "bits of a cached key / value element: 16, or 4 (transformer families with heads of 64, 128, "
+                                 "192 or 256: 9/32 of the memory and of the decode step's cache traffic)")
+    share_prompts: bool = opt(False, "rollouts run a prompt once and fork its cache into the samples of its group")
     reward_vocab_subset: int = opt(1024, "size of the seeded rewarded-token subset")
     reward_seed: int = opt(7, "seed of the rewarded subset / prompts")
     adv_eps: float = opt(1e-6, "epsilon in the group advantage normalisation")

@@ -1,8 +1,16 @@
-"""Attention over paged K / V caches: native kernels on CUDA, PyTorch restatements elsewhere (oracle / CPU path)."""
+"""Attention over paged K / V caches in 16 or 4 bits, rows into and out of them, copies of their pages: native kernels on
+CUDA, PyTorch restatements elsewhere (oracle / CPU path).
+
+The 4-bit cache (``csrc/q4.cuh`` has the byte order): a pool ``[num_blocks, kv_heads, block_size / 16, 18 * head_dim]`` uint8
+holds keys and values; every 32 neighbouring elements of a token's head share an fp16 scale, a code n in 0..15 stands for
+``scale * (n - 8)``. 4.5 bits an element, so a token costs 9/32 of its 16-bit rows."""
 
 from __future__ import annotations
 
-from typing import Optional
+import contextlib
+import ctypes
+import functools
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -12,7 +20,14 @@ from .native import call, dtype_code, ptr, stream_ptr
 P, I, L, F = native.P, native.I, native.L, native.F
 native.register("icb_kv_append", [P, P, P, P, P, I, I, L, L, P])
 native.register("icb_paged_decode", [P, L, P, P, P, P, P, P, I, I, I, I, I, I, F, I, P, P, I, P, I, I, I, P, L])
+native.register("icb_kv_append_q4", [P, P, P, P, L, I, I, I, L, L, L, I, P])
+native.register("icb_kv_read_q4", [P, P, P, P, L, I, I, I, L, I, P])
+native.register("icb_paged_decode_q4", [P, L, P, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, P])
+native.register("icb_copy_pages", [P, I, P, P, I, P])
 _SMS = None
+_HALF = (torch.bfloat16, torch.float16)
+Q4_GROUP = 32                                       # elements that share a scale
+Q4_HEAD_DIMS = (64, 128, 192, 256)
 
 
 def _decode_splits(rows: int, groups: int, max_tokens: int) -> int:
@@ -94,3 +109,250 @@ def paged_decode(q: torch.Tensor, k_cache, v_cache, block_table, seq_lens, hq: i
                  dtype_code(q.dtype), stream_ptr(), None, 0, None, 0, 0, 0, None, 0)
             return out
     return paged_decode_reference(q, k_cache, v_cache, block_table, seq_lens, hq, hkv, hd, scale)
+
+
+# --------------------------------------------------------------------------- pages
+def _on(t: torch.Tensor):
+    """Launches go to the tensor's device, whichever is current."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _page_numbers(x, name: str) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor):
+        if not all(isinstance(n, int) for n in x):
+            raise ValueError(f"{name} must be a list of page numbers")
+        x = torch.tensor(list(x), dtype=torch.int64)
+    if x.dim() != 1 or x.is_floating_point() or x.dtype == torch.bool:
+        raise ValueError(f"{name} must be a list of page numbers")
+    return x
+
+
+def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src, dst) -> None:
+    """Page ``dst[i]`` becomes page ``src[i]`` in every pool, all pools in one launch. ``pools``: one stacked tensor
+    [layers, pages, ...], or a sequence of tensors [pages, ...] (any shapes and types, contiguous). No page may be written
+    twice or be both written and read. ``src``, ``dst`` on the host (lists, CPU tensors) are checked for that and for their
+    range; int32 tensors on the device are taken as they are, pairs with a page outside a pool being left out."""
+    stacked = isinstance(pools, torch.Tensor)
+    tensors: List[torch.Tensor] = [pools] if stacked else list(pools)
+    src, dst = _page_numbers(src, "src"), _page_numbers(dst, "dst")
+    if src.numel() != dst.numel():
+        raise ValueError(f"{src.numel()} source pages for {dst.numel()} destinations")
+    if not tensors:
+        return
+    lead = 1 if stacked else 0
+    dev = tensors[0].device
+    for t in tensors:
+        if t.dim() <= lead or not t.is_contiguous():
+            raise ValueError("a pool must be contiguous, pages first" + (" after the layers" if stacked else ""))
+        if t.device != dev:
+            raise ValueError("the pools must be on one device")
+    pages = min(t.shape[lead] for t in tensors)
+    for x, other in ((src, dst), (dst, src)):
+        if x.is_cuda and (x.device != dev or other.device != dev or x.dtype != torch.int32):
+            raise ValueError("page numbers on the device must be int32, both on the pools' device")
+    if not src.is_cuda:
+        a, b = src.tolist(), dst.tolist()
+        if any(not 0 <= n < pages for n in a + b):
+            raise ValueError(f"page numbers must be in [0, {pages})")
+        if len(set(b)) != len(b) or not set(a).isdisjoint(b):
+            raise ValueError("a page may be written once, and not be read by another pair")
+    if src.numel() == 0:
+        return
+    if dev.type == "cuda":
+        with _on(tensors[0]):
+            src, dst = (x.to(dev, torch.int32).contiguous() for x in (src, dst))
+            records = []
+            for t in tensors:
+                if t.numel():
+                    size = t.element_size()
+                    records += [t.data_ptr(), t.shape[0] if stacked else 1, t.stride(0) * size if stacked else 0,
+                                t.shape[lead], t.stride(lead) * size]
+            if records:
+                call("icb_copy_pages", (ctypes.c_longlong * len(records))(*records), len(records) // 5, ptr(src), ptr(dst),
+                     src.numel(), stream_ptr())
+        return
+    a, b = src.long(), dst.long()
+    for t in tensors:
+        if stacked:
+            t[:, b] = t[:, a]
+        else:
+            t[b] = t[a]
+
+
+# --------------------------------------------------------------------------- the 4-bit cache
+def q4_pool_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int) -> Tuple[int, int, int, int]:
+    if block_size < 16 or block_size % 16:
+        raise ValueError("block_size must be a multiple of 16")
+    if head_dim not in Q4_HEAD_DIMS:
+        raise ValueError(f"a 4-bit cache holds heads of {', '.join(map(str, Q4_HEAD_DIMS))}, not {head_dim}")
+    return num_blocks, kv_heads, block_size // 16, 18 * head_dim
+
+
+def _q4_sizes(pool: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(blocks, kv heads, tiles of a page, head size) of a pool."""
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[3] % 18 or pool.shape[3] // 18 not in Q4_HEAD_DIMS \
+            or pool.shape[1] < 1 or pool.shape[2] < 1:
+        raise ValueError(f"not a 4-bit pool: {pool.dtype} {tuple(pool.shape)}")
+    if not pool.is_contiguous():
+        raise ValueError("a 4-bit pool must be contiguous")
+    return pool.shape[0], pool.shape[1], pool.shape[2], pool.shape[3] // 18
+
+
+def _same_device(pool: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != pool.device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """Rows that 16-byte loads can read: neighbouring elements, aligned starts."""
+    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 else x.contiguous()
+
+
+@functools.lru_cache(maxsize=16)
+def _q4_places(hd: int, device: torch.device) -> torch.Tensor:
+    """Byte of a tile for [token 0..15, byte]: hd / 2 bytes of key codes (elements 2 i, 2 i + 1), hd / 2 of value codes, the
+    scales."""
+    ng = hd // 32
+    t = torch.arange(16, device=device)[:, None]
+    d = torch.arange(0, hd, 2, device=device)[None, :]
+    word = (t // 8) * ng + d // 32
+    at = word // 4 * 512 + word % 4 * 4
+    keys = at + (4 * (t % 8) + d % 32 // 8) * 16 + d % 8 // 2
+    values = 8 * hd + at + (4 * (d % 32 // 4) + t % 8 // 2) * 16 + t % 2 * 2 + d % 4 // 2
+    return torch.cat((keys, values, 16 * hd + t * 4 * ng + torch.arange(4 * ng, device=device)), 1)
+
+
+def q4_quantize_reference(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [..., hd] -> codes uint8 [..., hd], scales fp16 [..., hd / 32]."""
+    g = x.float().unflatten(-1, (-1, Q4_GROUP))
+    most, least = g.amax(-1), g.amin(-1)
+    scale = (torch.where(most >= -least, most, least) / -8.0).clamp(-65504.0, 65504.0).half()
+    scale = torch.where(scale == 0, torch.zeros_like(scale), scale)
+    n = torch.round(g / scale.float().unsqueeze(-1)).clamp(-8.0, 7.0)
+    n = torch.where((scale == 0).unsqueeze(-1), torch.zeros_like(n), torch.nan_to_num(n, nan=0.0))
+    return (n + 8.0).to(torch.uint8).flatten(-2), scale
+
+
+def _q4_bytes_at(pool: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """Index of every byte of the rows ``slots`` (valid ones) in the flat pool: [T, kv heads, 9 hd / 8]."""
+    _, hkv, tiles, width = pool.shape
+    block, inside = slots // (16 * tiles), slots % (16 * tiles)
+    tile = (block[:, None] * hkv + torch.arange(hkv, device=pool.device)) * tiles + inside[:, None] // 16
+    return tile[..., None] * width + _q4_places(width // 18, pool.device)[inside % 16][:, None, :]
+
+
+def kv_append_q4_reference(k, v, pool, slots):
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    ok = (slots >= 0) & (slots < blocks * tiles * 16)
+    (kc, ks), (vc, vs) = (q4_quantize_reference(x[ok].unflatten(1, (hkv, hd))) for x in (k, v))
+    scales = torch.stack((ks, vs), 2).flatten(2).contiguous().view(torch.uint8)
+    pool.view(-1)[_q4_bytes_at(pool, slots[ok])] = torch.cat((kc[..., 0::2] | kc[..., 1::2] << 4,
+                                                              vc[..., 0::2] | vc[..., 1::2] << 4, scales), -1)
+
+
+def kv_read_q4_reference(pool, slots, dtype=torch.float32):
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    ok = (slots >= 0) & (slots < blocks * tiles * 16)
+    data = pool.view(-1)[_q4_bytes_at(pool, torch.where(ok, slots, torch.zeros_like(slots)))] if blocks else \
+        torch.zeros((slots.numel(), hkv, 9 * hd // 8), dtype=torch.uint8, device=pool.device)
+    n = torch.stack((data[..., :hd] & 15, data[..., :hd] >> 4), -1).flatten(-2).float() - 8.0
+    both = n * data[..., hd:].contiguous().view(torch.float16).float().repeat_interleave(Q4_GROUP, -1)
+    both = torch.where(ok[:, None, None], both, torch.zeros_like(both)).to(dtype)
+    return both[..., :hd].flatten(1), both[..., hd:].flatten(1)
+
+
+def paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs=None):
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    bs, out = 16 * tiles, torch.zeros((q.shape[0], hq * hd), dtype=q.dtype, device=q.device)
+    for i in range(q.shape[0]):
+        row = i if seqs is None else int(seqs[i])
+        n = min(int(seq_lens[i]), block_table.shape[1] * bs) if 0 <= row < block_table.shape[0] else 0
+        if n <= 0:
+            continue
+        tok = torch.arange(n, device=q.device)
+        page = block_table[row, tok // bs].long()
+        tok, page = tok[(page >= 0) & (page < blocks)], page[(page >= 0) & (page < blocks)]
+        if tok.numel() == 0:
+            continue
+        k, v = (x.view(-1, hkv, hd).repeat_interleave(hq // hkv, 1)
+                for x in kv_read_q4_reference(pool, page * bs + tok % bs))
+        p = torch.softmax(torch.einsum("hd,nhd->hn", q[i].view(hq, hd).float(), k) * scale, dim=-1)
+        out[i] = torch.einsum("hn,nhd->hd", p, v).reshape(-1).to(q.dtype)
+    return out
+
+
+def kv_append_q4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise k, v [T, hkv * hd] (row views with arbitrary pitch) and write them to the cache rows ``slots`` (int64 [T],
+    block * block_size + offset; rows with a slot outside the pool are left out). Two rows with one slot: either may win,
+    element by element."""
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    if k.dim() != 2 or k.shape != v.shape or k.shape[1] != hkv * hd or k.dtype != v.dtype:
+        raise ValueError(f"rows of {hkv} heads of {hd} expected, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if slots.dtype != torch.int64 or slots.shape != k.shape[:1]:
+        raise ValueError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
+    _same_device(pool, k=k, v=v, slots=slots)
+    if k.is_cuda and k.dtype in _HALF:
+        with _on(pool):
+            k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
+            call("icb_kv_append_q4", ptr(k), ptr(v), ptr(pool), ptr(slots), k.shape[0], hkv, hd, tiles, blocks * tiles * 16,
+                 k.stride(0), v.stride(0), dtype_code(k.dtype), stream_ptr())
+        return
+    kv_append_q4_reference(k, v, pool, slots)
+
+
+def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [T, hkv * hd] of the cache rows ``slots`` (int64 [T]); zeros for a slot outside the pool."""
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise ValueError(f"slots must be int64 [T], got {slots.dtype} {tuple(slots.shape)}")
+    if not dtype.is_floating_point:
+        raise ValueError(f"cannot read a cache as {dtype}")
+    _same_device(pool, slots=slots)
+    if pool.is_cuda and dtype in _HALF:
+        t = slots.numel()
+        with _on(pool):
+            k, v = torch.empty((2, t, hkv * hd), dtype=dtype, device=pool.device)
+            slots = slots.contiguous()
+            call("icb_kv_read_q4", ptr(pool), ptr(slots), ptr(k), ptr(v), t, hkv, hd, tiles, blocks * tiles * 16,
+                 dtype_code(dtype), stream_ptr())
+        return k, v
+    return kv_read_q4_reference(pool, slots, dtype)
+
+
+def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, hq: int,
+                    scale: Optional[float] = None, *, seqs: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, hq * hd] (row view, any pitch): row i against the first ``seq_lens[i]`` tokens of the sequence whose pages are
+    row ``seqs[i]`` of ``block_table`` (int32; None: row i) -> [T, hq * hd], into ``out`` (rows of any pitch) if given.
+    A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens."""
+    blocks, hkv, tiles, hd = _q4_sizes(pool)
+    t = q.shape[0]
+    scale = float(scale) if scale is not None else hd ** -0.5
+    if hq < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads do not share {hkv} key / value heads evenly")
+    if q.dim() != 2 or q.shape[1] != hq * hd:
+        raise ValueError(f"query rows of {hq} heads of {hd} expected, got {tuple(q.shape)}")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
+            or seq_lens.shape != (t,) or (seqs is not None and (seqs.dtype != torch.int32 or seqs.shape != (t,))):
+        raise ValueError("block_table [S, pages], seq_lens [T] and seqs [T] must be int32")
+    if seqs is None and block_table.shape[0] < t:
+        raise ValueError(f"{t} rows for {block_table.shape[0]} rows of pages")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(1) != 1):
+        raise ValueError("out must have q's shape and type and neighbouring elements")
+    _same_device(pool, q=q, block_table=block_table, seq_lens=seq_lens, seqs=seqs, out=out)
+    if q.is_cuda and q.dtype in _HALF:
+        with _on(pool):
+            if out is None:
+                out = torch.empty((t, hq * hd), dtype=q.dtype, device=q.device)
+            q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
+            seqs = seqs.contiguous() if seqs is not None else None
+            nsplit = _decode_splits(t, hkv * ((hq // hkv + 7) // 8), block_table.shape[1] * tiles * 16)
+            scratch = torch.empty(max(1, t * hq * nsplit * (hd + 2) if nsplit > 1 else 1), dtype=torch.float32, device=q.device)
+            call("icb_paged_decode_q4", ptr(q), q.stride(0), ptr(pool), ptr(block_table), ptr(seqs), ptr(seq_lens), ptr(out),
+                 out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, block_table.shape[1], block_table.shape[0], blocks, nsplit,
+                 scale, dtype_code(q.dtype), stream_ptr())
+        return out
+    res = paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs)
+    return res if out is None else out.copy_(res)

@@ -5,13 +5,19 @@ physical block of a sequence's i-th page and ``seq_lens[seq]`` its current lengt
 updated in place, so a captured CUDA graph of the decode step keeps reading the current state.
 
 * :class:`BlockKVCache` — keys and values, pools ``[num_blocks, block_size, kv_heads, head_dim]`` per layer.
-* :class:`LayerCache` — whatever the mixer of a layer run declares: rows per token, fixed-size states per sequence."""
+* :class:`QuantizedKVCache` — keys and values in 4 bits.
+* :class:`LayerCache` — whatever the mixer of a layer run declares: rows per token, fixed-size states per sequence.
+
+A sequence can be forked: its copies share its full pages, which nobody writes again, and get a last, partly filled page of
+their own. A page goes back to the free list when its last holder gives it back."""
 
 from __future__ import annotations
 
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import torch
+
+from ..ops import paged
 
 
 class PagedCache:
@@ -29,6 +35,7 @@ class PagedCache:
     # ---- sequences (host side) ----
     def reset(self):
         self._free: List[int] = list(range(self.num_blocks - 1, -1, -1))
+        self._holders = [0] * self.num_blocks            # sequences that have the page in their table
         self._owned: List[List[int]] = [[] for _ in range(self.max_seqs)]
         self._dropped = [0] * self.max_seqs              # leading pages given back because no layer can see them
         self._host_lens = [0] * self.max_seqs
@@ -58,6 +65,17 @@ class PagedCache:
     def free_blocks(self) -> int:
         return len(self._free)
 
+    def _take_page(self) -> int:
+        blk = self._free.pop()
+        self._holders[blk] = 1
+        return blk
+
+    def _give_back(self, blocks: Iterable[int]):
+        for blk in blocks:
+            self._holders[blk] -= 1
+            if self._holders[blk] == 0:
+                self._free.append(blk)
+
     def reserve(self, seq: int, new_len: int):
         """Make sure sequence ``seq`` owns enough pages for ``new_len`` tokens."""
         self.reserve_many([(seq, new_len)])
@@ -83,7 +101,7 @@ class PagedCache:
         rows, cols, blocks = [], [], []
         for seq, have, need in plan:
             for page in range(have, need):
-                blk = self._free.pop()
+                blk = self._take_page()
                 self._owned[seq].append(blk)
                 rows.append(seq)
                 cols.append(page)
@@ -96,16 +114,69 @@ class PagedCache:
         """Give back the pages of ``seq`` that end at or before ``position`` (no later token sees them)."""
         n = position // self.block_size - self._dropped[seq]
         if n > 0:
-            self._free.extend(reversed(self._owned[seq][:n]))
+            self._give_back(reversed(self._owned[seq][:n]))
             del self._owned[seq][:n]
             self._dropped[seq] += n
 
     def free(self, seq: int):
-        self._free.extend(reversed(self._owned[seq]))
+        self._give_back(reversed(self._owned[seq]))
         self._owned[seq] = []
         self._dropped[seq] = 0
         self._host_lens[seq] = 0
         self.seq_lens[seq] = 0
+
+    # ---- forks ----
+    def fork(self, seq: int, copies: int = 1) -> List[int]:
+        """Sequences from :meth:`acquire` that continue from what ``seq`` holds now; all or nothing. Pages that are full
+        are shared, the rest of its last page is copied, in every layer at once."""
+        return self.fork_many([seq], copies)[0]
+
+    def fork_many(self, seqs: Sequence[int], copies: int = 1) -> List[List[int]]:
+        """:meth:`fork` for several sequences with one copy and one table update."""
+        if copies < 0:
+            raise ValueError("copies must not be negative")
+        partial = [self._host_lens[s] % self.block_size > 0 for s in seqs]
+        if copies * len(seqs) > len(self._idle):
+            raise RuntimeError("not enough idle cache sequences to fork")
+        if copies * sum(partial) > len(self._free):
+            raise RuntimeError("KV cache is out of blocks")
+        parents, forks, src, dst, rows, cols, blocks = [], [], [], [], [], [], []
+        for s, part in zip(seqs, partial):
+            n = self._host_lens[s] // self.block_size             # full pages, the dropped ones among them
+            shared = self._owned[s][:n - self._dropped[s]]
+            mine = [self._idle.pop() for _ in range(copies)]
+            forks.append(mine)
+            for f in mine:
+                parents.append(s)
+                for blk in shared:
+                    self._holders[blk] += 1
+                self._owned[f] = list(shared)
+                self._dropped[f], self._host_lens[f] = self._dropped[s], self._host_lens[s]
+                if part:
+                    blk = self._take_page()
+                    src.append(self._owned[s][n - self._dropped[s]])
+                    dst.append(blk)
+                    self._owned[f].append(blk)
+                    rows.append(f)
+                    cols.append(n)
+                    blocks.append(blk)
+        if parents:
+            index = torch.tensor([parents, [f for mine in forks for f in mine]], dtype=torch.int64).to(self.device)
+            self.block_table[index[1]] = self.block_table[index[0]]
+            self.seq_lens[index[1]] = torch.tensor([self._host_lens[s] for s in parents], dtype=torch.int32).to(self.device)
+            self._copy_states(parents, [f for mine in forks for f in mine])
+        if rows:
+            at = torch.tensor([rows, cols, blocks], dtype=torch.int64).to(self.device)
+            self.block_table[at[0], at[1]] = at[2].to(torch.int32)
+            self._copy_pages(src, dst)
+        return forks
+
+    def _copy_pages(self, src: List[int], dst: List[int]):
+        """Page dst[i] becomes page src[i], in every layer."""
+        raise NotImplementedError
+
+    def _copy_states(self, src: List[int], dst: List[int]):
+        """What a sequence keeps outside of its pages."""
 
     # ---- slot mapping ----
     def slots_for(self, seq_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
@@ -130,6 +201,47 @@ class BlockKVCache(PagedCache):
 
     def bytes_per_token(self) -> int:
         return 2 * self.num_layers * self.kv_heads * self.head_dim * torch.empty((), dtype=self.dtype).element_size()
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
+        paged.kv_append(k, v, self.k[layer], self.v[layer], slots)
+
+    def attend(self, layer: int, q: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, hq: int) -> torch.Tensor:
+        return paged.paged_decode(q, self.k[layer], self.v[layer], tables, lens, hq, self.kv_heads, self.head_dim)
+
+    def _copy_pages(self, src, dst):
+        paged.copy_pages(self.k + self.v, src, dst)
+
+
+class QuantizedKVCache(PagedCache):
+    """Keys and values in 4 bits with an fp16 scale per 32 elements: 9/32 of the 16-bit cache's bytes. ``pool``
+    [layers, num_blocks, kv_heads, block_size / 16, 18 * head_dim] uint8; head sizes 64, 128, 192 and 256."""
+
+    def __init__(self, num_layers: int, kv_heads: int, head_dim: int, num_blocks: int, block_size: int = 16,
+                 max_seqs: int = 128, max_seq_len: int = 1024, device="cuda"):
+        shape = paged.q4_pool_shape(num_blocks, kv_heads, block_size, head_dim)
+        super().__init__(num_blocks, block_size, max_seqs, max_seq_len, device)
+        self.num_layers, self.kv_heads, self.head_dim = num_layers, kv_heads, head_dim
+        self.pool = torch.zeros((num_layers, *shape), dtype=torch.uint8, device=self.device)
+        self.layers = list(self.pool.unbind(0))
+
+    def bytes_per_token(self) -> int:
+        return self.num_layers * self.kv_heads * self.head_dim * 9 // 8
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
+        paged.kv_append_q4(k, v, self.layers[layer], slots)
+
+    def attend(self, layer: int, q: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, hq: int) -> torch.Tensor:
+        return paged.paged_decode_q4(q, self.layers[layer], tables, lens, hq)
+
+    def read(self, layer: int, seq: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [length, kv_heads * head_dim] of what a layer holds of ``seq`` (zeros for pages given back)."""
+        pos = torch.arange(self.length(seq), device=self.device)
+        slots = self.slots_for(torch.full_like(pos, seq), pos)
+        kept = pos >= self._dropped[seq] * self.block_size
+        return paged.kv_read_q4(self.layers[layer], torch.where(kept, slots, torch.full_like(slots, -1)), dtype)
+
+    def _copy_pages(self, src, dst):
+        paged.copy_pages(self.pool, src, dst)
 
 
 class LayerCache(PagedCache):
@@ -157,6 +269,12 @@ class LayerCache(PagedCache):
 
     def bytes_per_token(self) -> int:
         return sum(sum(s.rows.values()) for s in self.specs) * torch.empty((), dtype=self.dtype).element_size()
+
+    def _copy_pages(self, src, dst):
+        paged.copy_pages([t.view(self.num_blocks, self.block_size, -1) for run in self.rows for t in run.values()], src, dst)
+
+    def _copy_states(self, src, dst):
+        paged.copy_pages([t for run in self.states for t in run.values()], src, dst)
 
     def bytes_per_sequence(self) -> int:
         """Fixed-size states of one sequence."""

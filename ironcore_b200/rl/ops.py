@@ -6,7 +6,8 @@ import torch
 
 from ..ops import native
 from ..ops.native import call, ptr, stream_ptr
-from ..ops.paged import kv_append, paged_decode, paged_decode_reference  # noqa: F401
+from ..ops.paged import (copy_pages, kv_append, kv_append_q4, kv_read_q4, paged_decode, paged_decode_q4,  # noqa: F401
+                         paged_decode_q4_reference, paged_decode_reference)
 
 P, L, F = native.P, native.L, native.F
 native.register("icb_grpo_loss", [P, P, P, P, P, P, P, P, P, L, F, F, P])

@@ -13,9 +13,8 @@ import torch.distributed as dist
 from ..ops import functional as OF
 from ..ops import kernels
 from ..parallel import mesh
-from . import ops as RO
 from .batch import StepBatch
-from .kv_cache import BlockKVCache
+from .kv_cache import BlockKVCache, QuantizedKVCache
 
 
 def _all_reduce(x, group):
@@ -25,7 +24,7 @@ def _all_reduce(x, group):
 
 
 class TransformerProgram:
-    """The unified transformer on the block KV cache. Prompts run the flash attention kernel on the packed projections
+    """The unified transformer on the block KV cache (``rl.kv_cache_bits``: 16 or 4). Prompts run the flash attention kernel on the packed projections
     and scatter the rotated K / V rows into cache pages; all other rows append and attend over their pages. Tensor
     parallelism uses the plain (non sequence-parallel) layout, one all-reduce after each row-parallel projection."""
 
@@ -43,8 +42,11 @@ class TransformerProgram:
         self.layers = list(model.model.layers)
         first = next(model.parameters())
         blocks = num_blocks or max_seqs * ((max_seq_len + block_size - 1) // block_size)
-        self.cache = BlockKVCache(len(self.layers), self.hkv, self.hd, blocks, block_size, max_seqs, max_seq_len,
-                                  first.dtype, first.device)
+        sizes = (len(self.layers), self.hkv, self.hd, blocks, block_size, max_seqs, max_seq_len)
+        if config.rl.kv_cache_bits == 4:
+            self.cache = QuantizedKVCache(*sizes, device=first.device)
+        else:
+            self.cache = BlockKVCache(*sizes, first.dtype, first.device)
 
     def refresh(self):
         pass
@@ -133,13 +135,12 @@ class TransformerProgram:
 
         def attend(li, layer, qkv):
             qkv = self._rope_inplace(layer, qkv, t, seq_len, pos)
-            RO.kv_append(qkv[:, q_cols:q_cols + kv_cols], qkv[:, q_cols + kv_cols:], cache.k[li], cache.v[li],
-                         batch.slots)
+            cache.append(li, qkv[:, q_cols:q_cols + kv_cols], qkv[:, q_cols + kv_cols:], batch.slots)
             if prompt:
                 return OF.rope_attention(qkv, num_heads=self.hq, num_kv_heads=self.hkv, head_dim=self.hd,
                                          seq_len=seq_len, rope=None, causal=True, cu_seqlens=cu,
                                          fused=self.config.trainer.use_flash_attn)
-            return RO.paged_decode(qkv[:, :q_cols], cache.k[li], cache.v[li], tables, lens, self.hq, self.hkv, self.hd)
+            return cache.attend(li, qkv[:, :q_cols], tables, lens, self.hq)
 
         if prompt and batch.uniform:
             x = self._embed(batch.tokens.view(-1, seq_len))
@@ -163,6 +164,8 @@ class StreamProgram:
 
     def __init__(self, model, config, max_seqs: int, max_seq_len: int, block_size: Optional[int],
                  num_blocks: Optional[int]):
+        if config.rl.kv_cache_bits != 16:
+            raise ValueError("rl.kv_cache_bits: residual-stream models keep their caches in 16 bits")
         self.model = model
         table = model.embedding.word_embeddings.weight
         self.cache = model.model.make_cache(max_seqs, max_seq_len, block_size or self.PAGE, num_blocks,
@@ -178,4 +181,6 @@ class StreamProgram:
 def make_program(model, config, **kw):
     from ..models.families import STREAM_FAMILIES
 
+    if config.rl.kv_cache_bits not in (4, 16):
+        raise ValueError(f"rl.kv_cache_bits must be 16 or 4, not {config.rl.kv_cache_bits}")
     return (StreamProgram if model.family in STREAM_FAMILIES else TransformerProgram)(model, config, **kw)

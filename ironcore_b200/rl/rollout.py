@@ -61,6 +61,16 @@ class RolloutEngine:
             self.cache.release(self._requests.pop(i))
 
     @torch.no_grad()
+    def fork(self, rid: Hashable, new_ids: Sequence[Hashable]) -> None:
+        """Requests that go on, each in its own way, from what running request ``rid`` has seen so far: they share its
+        full cache pages and copy the rest."""
+        if rid not in self._requests:
+            raise ValueError(f"request {rid!r} is not running")
+        if len(set(new_ids)) != len(new_ids) or any(i in self._requests for i in new_ids):
+            raise ValueError("forks need ids that no running request has, each its own")
+        self._requests.update(zip(new_ids, self.cache.fork(self._requests[rid], len(new_ids))))
+
+    @torch.no_grad()
     def step(self, entries: Sequence[Tuple[Hashable, Sequence[int], Optional[Sequence[int]]]]) -> torch.Tensor:
         """``entries``: (request id, its next tokens, places among them whose logits are wanted; None = the last).
         An unknown id starts a request. Returns logits [wanted, V_local] in entry order, in a buffer that the next
@@ -197,13 +207,16 @@ class RolloutEngine:
     def generate(self, prompts: Union[torch.Tensor, Sequence[Sequence[int]]],
                  max_new_tokens: Union[int, Sequence[int]], temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 1.0, generator: Optional[torch.Generator] = None,
-                 stop_token: Optional[int] = None):
+                 stop_token: Optional[int] = None, samples: int = 1):
         """Sample continuations of a batch of prompts.
 
         ``prompts`` [S, P]: returns (tokens [S, P + N] including the prompt, log-probs of the N sampled tokens
         [S, N]). A list of token lists may be unequal, with one ``max_new_tokens`` or one per prompt and an optional
         ``stop_token``; it runs in waves of up to ``max_seqs`` prompts whose requests leave the batch as they finish,
-        and returns (list of sampled tokens, list of their log-probs)."""
+        and returns (list of sampled tokens, list of their log-probs). ``samples`` continuations of every prompt,
+        neighbours in the result ([S * samples, ...]): the prompt runs once and its cache is forked."""
+        if samples < 1 or samples > self.max_seqs:
+            raise ValueError(f"samples must be in [1, {self.max_seqs}], the engine's sequences")
         was_training = self.model.training
         self.model.eval()
         self.program.refresh()
@@ -211,12 +224,13 @@ class RolloutEngine:
             if isinstance(prompts, torch.Tensor):
                 if stop_token is not None or not isinstance(max_new_tokens, int):
                     raise ValueError("stop_token and per-prompt lengths need a list of prompts")
-                return self._generate_uniform(prompts, max_new_tokens, temperature, top_k, top_p, generator)
+                return self._generate_uniform(prompts, max_new_tokens, temperature, top_k, top_p, generator, samples)
             limits = [max_new_tokens] * len(prompts) if isinstance(max_new_tokens, int) else list(max_new_tokens)
             out, logps = [], []
-            for lo in range(0, len(prompts), self.max_seqs):
-                t, lp = self._generate_wave(prompts[lo:lo + self.max_seqs], limits[lo:lo + self.max_seqs], temperature,
-                                            top_k, top_p, generator, stop_token)
+            wave = self.max_seqs // samples
+            for lo in range(0, len(prompts), wave):
+                t, lp = self._generate_wave(prompts[lo:lo + wave], limits[lo:lo + wave], temperature, top_k, top_p, generator,
+                                            stop_token, samples)
                 out += t
                 logps += lp
             return out, logps
@@ -227,16 +241,21 @@ class RolloutEngine:
     def _acquire(self, n: int) -> List[int]:
         return [self.cache.acquire() for _ in range(n)]
 
-    def _generate_uniform(self, prompts, max_new_tokens, temperature, top_k, top_p, generator):
+    def _generate_uniform(self, prompts, max_new_tokens, temperature, top_k, top_p, generator, samples):
         s, p = prompts.shape
-        out = torch.empty((s, p + max_new_tokens), dtype=torch.int64, device=self.device)
-        out[:, :p] = prompts.to(self.device)
-        logps = torch.empty((s, max_new_tokens), dtype=torch.float32, device=self.device)
+        prompts = prompts.to(self.device)
+        out = torch.empty((s * samples, p + max_new_tokens), dtype=torch.int64, device=self.device)
+        out[:, :p] = prompts.repeat_interleave(samples, dim=0) if samples > 1 else prompts
+        logps = torch.empty((s * samples, max_new_tokens), dtype=torch.float32, device=self.device)
         if max_new_tokens == 0:
             return out, logps
         seqs = self._acquire(s)
         try:
-            logits = self._rows(seqs, [p] * s, out[:, :p].reshape(-1), [(i + 1) * p - 1 for i in range(s)])
+            logits = self._rows(seqs, [p] * s, prompts.reshape(-1), [(i + 1) * p - 1 for i in range(s)])
+            if samples > 1:
+                forks = self.cache.fork_many(seqs, samples - 1)
+                seqs = [q for parent, mine in zip(seqs, forks) for q in (parent, *mine)]
+                logits = logits.repeat_interleave(samples, dim=0)
             for i in range(max_new_tokens):
                 tok, lp = self._sample(logits, temperature, top_k, top_p, generator)
                 out[:, p + i] = tok
@@ -248,14 +267,25 @@ class RolloutEngine:
                 self.cache.release(q)
         return out, logps
 
-    def _generate_wave(self, prompts, limits, temperature, top_k, top_p, generator, stop_token):
-        n = len(prompts)
+    def _generate_wave(self, prompts, limits, temperature, top_k, top_p, generator, stop_token, samples=1):
+        n = len(prompts) * samples
+        limits = [x for x in limits for _ in range(samples)]
         tokens: List[List[int]] = [[] for _ in range(n)]
         logps: List[List[float]] = [[] for _ in range(n)]
         live = [i for i in range(n) if limits[i] > 0]
         if not live:
             return tokens, logps
-        logits = self.step([(("wave", i), prompts[i], None) for i in live])
+        if samples > 1:
+            first = [i for i in live if i % samples == 0]
+            logits = self.step([(("wave", i), prompts[i // samples], None) for i in first]).repeat_interleave(samples, dim=0)
+            try:
+                for i in first:
+                    self.fork(("wave", i), [("wave", j) for j in range(i + 1, i + samples)])
+            except Exception:
+                self.end([("wave", i) for i in live if ("wave", i) in self._requests])
+                raise
+        else:
+            logits = self.step([(("wave", i), prompts[i], None) for i in live])
         while live:
             tok, lp = self._sample(logits, temperature, top_k, top_p, generator)
             done = []

@@ -61,7 +61,7 @@ class GRPOTrainer(Trainer):
         if mesh.get_tensor_model_parallel_world_size() > 1:
             base = base.to(self.device)
             dist.broadcast(base, src=mesh.get_tensor_model_parallel_src_rank(), group=mesh.get_tensor_model_parallel_group())
-        return base.repeat_interleave(rl.group_size, dim=0)
+        return base if rl.share_prompts else base.repeat_interleave(rl.group_size, dim=0)
 
     @torch.no_grad()
     def rollout(self) -> Dict[str, torch.Tensor]:
@@ -76,7 +76,7 @@ class GRPOTrainer(Trainer):
             e0.record()
         t0 = time.perf_counter()
         tokens, logp_old = self.engine.generate(prompts, rl.max_new_tokens, rl.temperature, rl.top_k, rl.top_p,
-                                                self.sample_gen)
+                                                self.sample_gen, samples=rl.group_size if rl.share_prompts else 1)
         if cuda:
             e1.record()
             e1.synchronize()

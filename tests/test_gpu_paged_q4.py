@@ -1,0 +1,340 @@
+"""Kernels of the 4-bit paged cache and of page copies against the definition in 64 bits."""
+
+import pytest
+import torch
+
+import q4_oracle as O
+from helpers import tiny_config
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _rows(t, hkv, hd, dtype, seed=0, device="cuda"):
+    """k, v as views of a packed projection, with groups of every kind among them."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((t, 3 * hkv * hd), generator=g) * 2.0 ** (16 * torch.rand((t, 3 * hkv * hd // 32), generator=g) - 8
+                                                            ).repeat_interleave(32, 1)
+    x = x.to(dtype)
+    k, v = x[:, hkv * hd:2 * hkv * hd], x[:, 2 * hkv * hd:]
+    k[0, :32] = 0
+    v[t // 2] = torch.tensor([1.0, -1.0]).to(dtype).repeat(hkv * hd // 2)
+    k[t - 1, :64] = torch.arange(-32, 32).to(dtype) / 4                      # quotients that are ties
+    x = x.to(device)
+    return x[:, hkv * hd:2 * hkv * hd], x[:, 2 * hkv * hd:]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hkv,hd,bs,t", [(2, 128, 16, 1), (12, 64, 32, 77), (1, 256, 16, 300), (3, 192, 48, 130), (8, 128, 64, 1000)])
+def test_append_and_read(hkv, hd, bs, t, dtype):
+    from ironcore_b200.ops import paged
+
+    k, v = _rows(t, hkv, hd, dtype)
+    blocks = -(-t // bs) + 3
+    g = torch.Generator().manual_seed(1)
+    start = torch.randint(0, 255, paged.q4_pool_shape(blocks, hkv, bs, hd), dtype=torch.uint8, generator=g)
+    order = torch.randperm(blocks, generator=g)
+    first = 5 % bs if t < blocks * bs - 5 else 0
+    for name, slots in (("scattered", torch.randperm(blocks * bs, generator=g)[:t]),
+                        ("in order", order[(torch.arange(t) + first) // bs] * bs + (torch.arange(t) + first) % bs),
+                        ("some left out", torch.where(torch.rand(t, generator=g) < 0.3, -torch.ones(t, dtype=torch.int64),
+                                                      order[torch.arange(t) // bs] * bs + torch.arange(t) % bs))):
+        if t > 3 and name == "some left out":
+            slots[1], slots[2] = blocks * bs, 2 ** 40
+        want, got = start.clone(), start.clone().cuda()
+        paged.kv_append_q4_reference(k.cpu(), v.cpu(), want, slots)
+        paged.kv_append_q4(k, v, got, slots.cuda())
+        assert torch.equal(got.cpu(), want), name
+        for x, y in zip(paged.kv_read_q4(got, slots.cuda(), dtype), paged.kv_read_q4_reference(want, slots, dtype)):
+            assert torch.equal(x.cpu().nan_to_num(), y.nan_to_num()), name
+    # every row of the pool, stale ones included, in order and with both ends beyond it
+    every = torch.arange(-3, blocks * bs + 5)
+    for x, y in zip(paged.kv_read_q4(got, every.cuda(), dtype), paged.kv_read_q4_reference(want, every, dtype)):
+        assert torch.equal(x.cpu().nan_to_num(), y.nan_to_num()) and torch.equal(x.cpu().isnan(), y.isnan())
+
+
+def test_append_extreme_groups():
+    from ironcore_b200.ops import paged
+
+    for dtype, big in ((BF, 3e38), (HF, 65504.0)):
+        k = torch.ones((7, 64), dtype=dtype)
+        k[0, :32] = 0
+        k[1, :32] = torch.tensor([1e-38, -1e-39] * 16).to(dtype)
+        k[2, 3] = big
+        k[3, 5] = float("-inf")
+        k[4, 7] = float("nan")
+        k[5, :32] = torch.tensor([2.0, -2.0] * 16)
+        k[6, 0] = -1.0
+        want = torch.zeros(paged.q4_pool_shape(1, 1, 16, 64), dtype=torch.uint8)
+        got = want.cuda()
+        paged.kv_append_q4_reference(k, k, want, torch.arange(7))
+        paged.kv_append_q4(k.cuda(), k.cuda(), got, torch.arange(7).cuda())
+        for x, y in zip(paged.kv_read_q4(got, torch.arange(7).cuda(), BF), paged.kv_read_q4_reference(want, torch.arange(7), BF)):
+            assert torch.equal(x.cpu().nan_to_num(7.0), y.nan_to_num(7.0))
+        codes = 16 * 64                                     # NaN scales may differ in their bits, codes may not
+        assert torch.equal(got.cpu()[..., :codes], want[..., :codes])
+
+
+def _check(q, pool, table, lens, hq, scale=None, **kw):
+    from ironcore_b200.ops import paged
+
+    hd = pool.shape[3] // 18
+    out = paged.paged_decode_q4(q, pool, table, lens, hq, scale, **kw)
+    want, tol = O.attention(q.cpu(), *O.decoded(pool), table.cpu(), lens.cpu(), hq, scale or O.scale_of(hd),
+                            kw["seqs"].cpu() if "seqs" in kw else None)
+    off = (out.cpu().double() - want).abs()
+    assert bool(torch.isfinite(out).all())
+    assert bool((off <= tol).all()), f"{float((off / tol).max()):.2f} of the tolerance"
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hq,hkv,hd,bs", [(2, 1, 64, 16), (12, 2, 128, 16), (12, 12, 64, 64), (8, 1, 256, 32), (16, 1, 128, 16),
+                                          (11, 1, 192, 48), (10, 2, 64, 16), (32, 8, 128, 64)])
+def test_attention(hq, hkv, hd, bs, dtype):
+    lens = [1, 0, 15, 16, 17, 33, 2 * bs, 2 * bs + 1, 200, 129]
+    pool, table, lens = O.cache(lens, hkv, hd, bs, dtype, seed=hq, device="cuda")
+    q = (2 * torch.randn((10, (hq + 2 * hkv) * hd), generator=torch.Generator().manual_seed(1))).to(dtype).cuda()[:, :hq * hd]
+    out = _check(q, pool, table, lens, hq)
+    assert not out[1].any()
+
+
+@pytest.mark.parametrize("spread", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_over_long_contexts(hd, spread):
+    pool, table, lens = O.cache([9000, 3, 0, 2777, 5000], 2, hd, 16, BF, seed=5, spread=spread, device="cuda")
+    q = torch.randn((5, 6 * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    _check(q, pool, table, lens, 6)
+
+
+def test_attention_with_one_dominant_token():
+    """A first token that takes nearly all probability and has tiny values, among values of ordinary size."""
+    from ironcore_b200.ops import paged
+
+    hd, n = 128, 2500
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn((n + 12, hd), generator=g) for _ in range(2))
+    q = torch.randn((1, hd), generator=g)
+    k[0] = q[0]
+    v[0] *= 2.0 ** -13
+    pool = torch.zeros(paged.q4_pool_shape(157, 1, 16, hd), dtype=torch.uint8)
+    paged.kv_append_q4_reference(k.to(BF), v.to(BF), pool, torch.arange(n + 12))
+    table, lens = torch.arange(157, dtype=torch.int32)[None].cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    for factor in (0.05, 0.15, 1.0):
+        _check(q.to(BF).cuda(), pool.cuda(), table, lens, 1, factor)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -60, 1.0, 2.0 ** 60])
+def test_attention_with_queries_of_any_size(size):
+    pool, table, lens = O.cache([77, 300], 1, 128, 16, BF, seed=2, device="cuda")
+    q = torch.randn((2, 4 * 128), generator=torch.Generator().manual_seed(1))
+    q[0, 3:60] *= 2.0 ** -20                                # small elements beside large ones
+    _check((q * size).to(BF).cuda(), pool, table, lens, 4, 0.09 / size)
+
+
+def test_attention_over_stale_pages():
+    """NaN scales and any codes behind the last token, in unused pages and in pages of other sequences."""
+    hkv, hd, bs = 2, 128, 32
+    lens = [1, 17, 40, 0, 64]
+    pool, table, dev_lens = O.cache(lens, hkv, hd, bs, BF, seed=3)
+    stale = torch.ones((pool.shape[0], bs), dtype=torch.bool)
+    for i, n in enumerate(lens):
+        for p in range(n):
+            stale[table[i, p // bs], p % bs] = False
+    half = pool[..., 16 * hd:].contiguous().view(torch.float16).view(-1, hkv, bs // 16, 16, 8)
+    mask = stale.view(-1, 1, bs // 16, 16, 1).expand_as(half)
+    half = torch.where(mask, torch.tensor(float("nan"), dtype=HF), half)
+    pool[..., 16 * hd:] = half.view(pool.shape[0], hkv, bs // 16, 128).contiguous().view(torch.uint8)
+    q = torch.randn((5, 4 * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    from ironcore_b200.ops import paged
+
+    out = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)
+    k, v = O.decoded(pool)
+    want, tol = O.attention(q.cpu(), k.nan_to_num(), v.nan_to_num(), table, dev_lens, 4, O.scale_of(hd))
+    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+    # a NaN among the tokens does reach its sequence, and no other
+    row = pool[table[1, 0], 0, 0, 16 * hd:].view(torch.float16)
+    row[0] = float("nan")
+    again = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)
+    assert again[1, :2 * hd].isnan().all() and torch.equal(again[[0, 2, 3, 4]], out[[0, 2, 3, 4]])
+    assert torch.equal(again[1, 2 * hd:], out[1, 2 * hd:])
+
+
+def test_attention_calls_of_every_form():
+    """Rows that name their sequence, one sequence several times, outputs and queries of odd pitch and alignment, page
+    numbers and rows outside, lengths beyond the table."""
+    from ironcore_b200.ops import paged
+
+    hkv, hd, bs, hq = 2, 64, 16, 6
+    pool, table, _ = O.cache([100, 60, 90], hkv, hd, bs, HF, seed=4)
+    table[1, 1], table[2, 0] = -1, pool.shape[0]
+    seqs = torch.tensor([2, 0, 0, 0, 1, 3, -1, 0], dtype=torch.int32).cuda()
+    lens = torch.tensor([90, 100, 1, 50, 60, 9, 9, 10 ** 9], dtype=torch.int32).cuda()
+    assert table.shape[1] * bs == 112
+    table[0, 6] = table[0, 5]                               # the whole row of the table holds pages
+    wide = torch.randn((8, hq * hd + 24), generator=torch.Generator().manual_seed(1)).to(HF).cuda()
+    pool, table = pool.cuda(), table.cuda()
+    first = _check(wide[:, :hq * hd], pool, table, lens, hq, seqs=seqs)
+    assert not first[5].any() and not first[6].any()
+    for lo in (1, 8, 3):
+        _check(wide[:, lo:lo + hq * hd], pool, table, lens, hq, seqs=seqs)
+    into = torch.full((8, hq * hd + 3), 9.0, dtype=HF, device="cuda")
+    paged.paged_decode_q4(wide[:, :hq * hd], pool, table, lens, hq, seqs=seqs, out=into[:, 1:1 + hq * hd])
+    assert torch.equal(into[:, 1:1 + hq * hd], first) and bool((into[:, 0] == 9).all()) and bool((into[:, -2:] == 9).all())
+    assert paged.paged_decode_q4(wide[:0, :hq * hd], pool, table, lens[:0], hq).shape == (0, hq * hd)
+    nothing = paged.paged_decode_q4(wide[:, :hq * hd], pool, table[:, :0], lens, hq, seqs=seqs)
+    assert not nothing.any()
+
+
+def test_attention_is_reproducible_and_runs_on_other_streams():
+    from ironcore_b200.ops import paged
+
+    pool, table, lens = O.cache([1500, 700, 3, 0, 999], 4, 128, 16, BF, seed=6, device="cuda")
+    q = torch.randn((5, 16 * 128), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    first = paged.paged_decode_q4(q, pool, table, lens, 16)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(paged.paged_decode_q4(q, pool, table, lens, 16))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+
+
+def test_attention_in_graphs():
+    """Two captured calls that share nothing, replayed in turn with lengths that change between replays."""
+    from ironcore_b200.ops import paged
+
+    sets = []
+    for seed, hd in ((7, 128), (8, 64)):
+        pool, table, lens = O.cache([800, 50, 300], 2, hd, 16, BF, seed=seed, device="cuda")
+        q = torch.randn((3, 8 * hd), generator=torch.Generator().manual_seed(seed)).to(BF).cuda()
+        paged.paged_decode_q4(q, pool, table, lens, 8)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged.paged_decode_q4(q, pool, table, lens, 8)
+        sets.append((q, pool, table, lens, graph, out))
+    for now in ([800, 50, 300], [1, 0, 299], [17, 49, 0], [799, 16, 1]):
+        for q, pool, table, lens, graph, out in sets:
+            lens.copy_(torch.tensor(now, dtype=torch.int32))
+            out.fill_(float("nan"))
+        for _ in range(2):
+            for s in sets:
+                s[4].replay()
+        for q, pool, table, lens, graph, out in sets:
+            assert torch.equal(out, paged.paged_decode_q4(q, pool, table, lens, 8))
+    q, pool, table, lens, graph, out = sets[0]
+    want, tol = O.attention(q.cpu(), *O.decoded(pool), table.cpu(), lens.cpu(), 8, O.scale_of(128))
+    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+
+
+def test_pools_larger_than_32_bit_offsets():
+    """Pages on both sides of 2^31 and 2^32 bytes."""
+    from ironcore_b200.ops import paged
+
+    hkv, hd, bs = 8, 128, 64
+    size = hkv * hd * 18 // 16 * bs
+    blocks = 2 ** 32 // size + 3
+    pool = torch.empty(paged.q4_pool_shape(blocks, hkv, bs, hd), dtype=torch.uint8, device="cuda")
+    pages = torch.tensor([blocks - 1, 0, 2 ** 31 // size, blocks - 2, 2 ** 32 // size])
+    k, v = _rows(5 * bs, hkv, hd, BF, seed=2)
+    slots = (pages[:, None] * bs + torch.arange(bs)).flatten().cuda()
+    small = torch.zeros(paged.q4_pool_shape(5, hkv, bs, hd), dtype=torch.uint8, device="cuda")
+    paged.kv_append_q4(k, v, pool, slots)
+    paged.kv_append_q4(k, v, small, torch.arange(5 * bs).cuda())
+    assert torch.equal(pool[pages.cuda()], small)
+    for x, y in zip(paged.kv_read_q4(pool, slots), paged.kv_read_q4(small, torch.arange(5 * bs).cuda())):
+        assert torch.equal(x, y)
+    q = torch.randn((1, 16 * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    lens = torch.tensor([5 * bs - 7], dtype=torch.int32).cuda()
+    assert torch.equal(paged.paged_decode_q4(q, pool, pages[None].int().cuda(), lens, 16),
+                       paged.paged_decode_q4(q, small, torch.arange(5, dtype=torch.int32)[None].cuda(), lens, 16))
+    paged.copy_pages([pool], [blocks - 1], [1])
+    assert torch.equal(pool[1], small[0])
+
+
+def test_copy_pages_kernel():
+    from ironcore_b200.ops import paged
+
+    g = torch.Generator().manual_seed(0)
+    shapes = [((40, 16, 2, 64), BF), ((40, 5), torch.float32), ((41, 3), torch.uint8), ((40, 1, 7), HF), ((40, 33000), torch.uint8),
+              ((40, 0), BF), ((50, 4096), torch.float32)]
+    pools = [(100 * torch.randn(s, generator=g)).to(t) for s, t in shapes] * 15          # more than one launch
+    dev = [p.cuda() for p in pools]
+    src, dst = [3, 3, 0, 39], [1, 38, 2, 10]
+    paged.copy_pages(dev, src, dst)
+    for p, d in zip(pools, dev):
+        p = p.clone()
+        p[dst] = p[src]
+        assert torch.equal(p, d.cpu())
+    stack = torch.randint(0, 255, (3, 20, 2, 1, 18 * 64), dtype=torch.uint8, generator=g)
+    got = stack.cuda()
+    # device lists: pairs outside the pool are left out
+    paged.copy_pages(got, torch.tensor([4, -1, 5, 20, 6], dtype=torch.int32).cuda(),
+                     torch.tensor([0, 1, 20, 2, 19], dtype=torch.int32).cuda())
+    stack[:, [0, 19]] = stack[:, [4, 6]]
+    assert torch.equal(stack, got.cpu())
+    views = torch.zeros((9, 5), dtype=torch.uint8, device="cuda").view(-1)[1:41].view(8, 5)      # odd addresses
+    views[2] = torch.arange(5)
+    paged.copy_pages([views], [2], [7])
+    assert views[7].tolist() == [0, 1, 2, 3, 4] and int(views.sum()) == 20
+    with pytest.raises(ValueError):
+        paged.copy_pages(got, torch.tensor([4]).cuda(), torch.tensor([0]).cuda())
+    with pytest.raises(ValueError):
+        paged.copy_pages(got, torch.tensor([4], dtype=torch.int32).cuda(), [0])
+
+
+def test_refusals_on_the_gpu():
+    from ironcore_b200.ops import paged
+
+    pool = torch.zeros(paged.q4_pool_shape(2, 2, 16, 64), dtype=torch.uint8, device="cuda")
+    rows, slots = torch.zeros((3, 128), dtype=BF, device="cuda"), torch.arange(3, device="cuda")
+    for bad in ((rows.cpu(), rows.cpu(), slots), (rows, rows, slots.cpu())):
+        with pytest.raises(ValueError):
+            paged.kv_append_q4(bad[0], bad[1], pool, bad[2])
+    q = torch.zeros((3, 256), dtype=BF, device="cuda")
+    table, lens = torch.zeros((3, 1), dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for kw in (dict(q=q.cpu()), dict(block_table=table.cpu()), dict(seq_lens=lens.cpu()), dict(seqs=lens.cpu())):
+        with pytest.raises(ValueError):
+            paged.paged_decode_q4(**{**dict(q=q, pool=pool, block_table=table, seq_lens=lens, hq=4), **kw})
+    with pytest.raises(ValueError):
+        paged.kv_read_q4(pool, slots.cpu())
+    # fp32 rows run on PyTorch operators
+    k = torch.randn((3, 128), generator=torch.Generator().manual_seed(0))
+    paged.kv_append_q4(k.cuda(), k.cuda(), pool, slots)
+    assert torch.equal(paged.kv_read_q4(pool, slots, torch.float32)[0].cpu().double(), O.quantised(k.view(3, 2, 64)).flatten(1))
+
+
+def _engine(bits, **kw):
+    from ironcore_b200.config import validate_config
+    from ironcore_b200.models import LanguageModel
+    from ironcore_b200.parallel import mesh
+    from ironcore_b200.rl import RolloutEngine
+
+    mesh.destroy_model_parallel()
+    cfg = tiny_config("qwen", d_model=256, d_ffn=512, num_layers=2, num_attention_heads=4, num_attention_groups=2, head_dim=128,
+                      max_seq_len=128, max_position_embeddings=128, precision="bf16", vocab_size=1024, qkv_bias=True)
+    cfg.data.vocab_size = 1024
+    cfg.rl.kv_cache_bits = bits
+    validate_config(cfg)
+    torch.manual_seed(3)
+    model = LanguageModel(cfg, device=torch.device("cuda")).cuda().eval()
+    return model, RolloutEngine(model, cfg, max_seqs=6, max_seq_len=128, **kw)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_rollouts(bits):
+    """The whole path: prompt, quantised rows, captured decode steps, forks."""
+    prompts = torch.randint(0, 1024, (2, 37), generator=torch.Generator().manual_seed(1))
+    model, eager = _engine(bits, use_cuda_graph=False)
+    t1, lp1 = eager.generate(prompts.repeat_interleave(3, dim=0), 24, temperature=0.0)
+    _, graph = _engine(bits, use_cuda_graph=True)
+    t2, lp2 = graph.generate(prompts, 24, temperature=0.0, samples=3)
+    assert graph.cache.free_blocks == graph.cache.num_blocks
+    full = model.token_logprobs(t1[:, :-1], t1[:, 1:])[:, 36:]
+    assert bool(torch.isfinite(lp1).all()) and (full - lp1).abs().max().item() < (0.5 if bits == 4 else 0.15)
+    assert t2.shape == t1.shape and torch.equal(t2[0], t2[1]) and torch.equal(t2[0], t2[2])
+    again, lp3 = graph.generate(prompts, 24, temperature=0.0, samples=3)
+    assert torch.equal(t2, again) and torch.equal(lp2, lp3)
