@@ -23,6 +23,7 @@ native.register("icb_paged_decode", [P, L, P, P, P, P, P, P, I, I, I, I, I, I, F
 native.register("icb_kv_append_q4", [P, P, P, P, L, I, I, I, L, L, L, I, P])
 native.register("icb_kv_read_q4", [P, P, P, P, L, I, I, I, L, I, P])
 native.register("icb_paged_decode_q4", [P, L, P, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, P])
+native.register("icb_paged_decode_q4_workers", [I, I])
 native.register("icb_copy_pages", [P, I, P, P, I, P])
 _SMS = None
 _HALF = (torch.bfloat16, torch.float16)
@@ -210,6 +211,15 @@ def _rows16(x: torch.Tensor) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=16)
+def _q4_workers(hd: int, dtype: torch.dtype) -> int:
+    """Blocks of the attention kernel that the GPU holds at a time."""
+    n = native.query("icb_paged_decode_q4_workers", hd, dtype_code(dtype))
+    if n < 1:
+        raise RuntimeError(f"icb_paged_decode_q4_workers failed with code {n}")
+    return n
+
+
+@functools.lru_cache(maxsize=16)
 def _q4_places(hd: int, device: torch.device) -> torch.Tensor:
     """Byte of a tile for [token 0..15, byte]: hd / 2 bytes of key codes (elements 2 i, 2 i + 1), hd / 2 of value codes, the
     scales."""
@@ -348,10 +358,12 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
                 out = torch.empty((t, hq * hd), dtype=q.dtype, device=q.device)
             q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
             seqs = seqs.contiguous() if seqs is not None else None
-            nsplit = _decode_splits(t, hkv * ((hq // hkv + 7) // 8), block_table.shape[1] * tiles * 16)
-            scratch = torch.empty(max(1, t * hq * nsplit * (hd + 2) if nsplit > 1 else 1), dtype=torch.float32, device=q.device)
+            # at most a worker for every four tiles of 16 tokens that the table has room for
+            most = t * block_table.shape[1] * tiles * hkv * ((hq // hkv + 7) // 8)
+            workers = max(1, min(_q4_workers(hd, q.dtype), most // 4))
+            scratch = torch.empty(workers * 16 * (hd + 4), dtype=torch.float32, device=q.device)
             call("icb_paged_decode_q4", ptr(q), q.stride(0), ptr(pool), ptr(block_table), ptr(seqs), ptr(seq_lens), ptr(out),
-                 out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, block_table.shape[1], block_table.shape[0], blocks, nsplit,
+                 out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, block_table.shape[1], block_table.shape[0], blocks, workers,
                  scale, dtype_code(q.dtype), stream_ptr())
         return out
     res = paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs)

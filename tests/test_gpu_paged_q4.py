@@ -158,6 +158,9 @@ def test_attention_over_stale_pages():
     again = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)
     assert again[1, :2 * hd].isnan().all() and torch.equal(again[[0, 2, 3, 4]], out[[0, 2, 3, 4]])
     assert torch.equal(again[1, 2 * hd:], out[1, 2 * hd:])
+    pool[table[0, 0], 1, 0, 16 * hd:16 * hd + 2] = torch.tensor([float("nan")], dtype=HF).view(torch.uint8)
+    again = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)          # the only token of a sequence
+    assert again[0, 2 * hd:].isnan().all() and torch.equal(again[0, :2 * hd], out[0, :2 * hd])
 
 
 def test_attention_calls_of_every_form():
