@@ -7,8 +7,9 @@
 //   * A code needs no conversion: four bits at the bottom of an fp16 are the number n 2^-24, exact in the matrix
 //     instruction, so a word & 0x000f000f is two operands, & 0x00f000f0 two more that are 16 n 2^-24. The factor 16 is taken
 //     out of the query elements beforehand and out of the output rows at the end; shifted by 8 the word gives the other four.
-//   * The -8 enters through the first addend: q . (n - 8) = q . n - 8 sum q per group, a constant of the query. On the value
-//     side a matrix instruction with a constant operand sums -8 p_t sv_tg from the same rounded products.
+//   * q . (n - 8) = q . n - 8 sum q: the second part is a product of the key scales with a constant of the query, one matrix
+//     instruction for all groups (the constant as fp16 plus what fp16 leaves of it, 22 bits). On the value side another one,
+//     whose constant operand has -8 in row g, sums -8 p_t sv_tg from the same rounded products.
 //   * The scale of a group multiplies a finished dot product (keys) or the probability before it is rounded to fp16 (values).
 //   * Queries are scaled per head by a power of two to [2^14, 2^15) so that bf16 fits fp16: an element loses bits only below
 //     2^-24 of the head's largest.
@@ -25,9 +26,11 @@ namespace icb {
 
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = kQ4Warps * 32;
-constexpr int kQ4MinTiles = kQ4Warps;           // a worker has at least a tile for each warp
+constexpr int kQ4MinTiles = 2;                  // least tiles of a warp
+constexpr int kQ4Whole = 8;                     // units of at most so many tiles are not divided among warps
 constexpr float kQ4Top = 12.f;                  // log2 of the largest fp16 probability times scale right after a new maximum
-constexpr float kQ4Slack = 3.f;                 // and how far it may grow before the maximum is taken again: 2^15 fits fp16
+constexpr float kQ4Limit = 32768.f;             // and what it may grow to before the maximum is taken again: fp16 holds it
+constexpr float kQ4None = -1e30f;               // maximum of no tokens
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Q4DecodeArgs {
@@ -39,9 +42,9 @@ struct Q4DecodeArgs {
   const int* lens;
   uint16_t* out;                // [rows, out_stride], heads HD apart
   long long out_stride;
-  float* part;                  // [workers][2][8] records of HD + 4 floats: outputs, maximum, sum
-  int rows, hq, hkv, slices, tiles, max_blocks, table_rows, num_blocks, workers;
-  uint32_t tiles_inverse;       // ceil(2^32 / tiles)
+  int4* owner;                  // [workers]: {row, unit, last worker} of a unit that begins in a worker's range and goes on
+  float* part;                  // [workers][2][slice heads] records of HD + 4 floats: outputs, maximum, sum
+  int rows, hq, hkv, slices, heads, tiles, max_blocks, table_rows, num_blocks;   // heads: of a slice, at most eight
   float scale;                  // score factor times log2(e)
 };
 
@@ -50,6 +53,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -63,11 +72,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ float log2_fast(float x) {
   float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void copy16(void* smem, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+__device__ __forceinline__ void copy16(uint32_t smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(global) : "memory");
 }
 
 template <bool BF16>
@@ -90,12 +99,12 @@ __device__ __forceinline__ void q4_store4(uint16_t* to, float x, float y, float 
 template <int NG>
 struct Q4Query {
   uint32_t b[NG][4];            // B fragments of the two matrix instructions of a group
-  float start[NG][2];           // -8 * sum of the group's query elements (in units of 2^-24), heads 2c and 2c + 1
-  float factor[2];              // from the sums to the base-2 score
+  uint32_t start[NG > 4 ? 2 : 1];   // B fragment of -8 * sum of a group's query elements: fp16 and what it leaves
+  float factor[2], factor8[2];  // from the dot products, and from the sums of `start`, to the base-2 score; heads 2c, 2c + 1
 };
 
 template <int NG, bool BF16>
-__device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint16_t* q, int heads, float scale) {
+__device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, int heads, float scale) {
   constexpr int HD = NG * 32;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   float x[NG][8];
@@ -103,7 +112,7 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint16_t* q,
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (r < heads) u = *reinterpret_cast<const uint4*>(q + r * HD + g * 32 + c * 8);
+    if (r < heads) u = *reinterpret_cast<const uint4*>(q + (r * HD + g * 32 + c * 8) * 2);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -118,6 +127,7 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint16_t* q,
   const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 116);
   const float up = __int_as_float((127 + 14 - e) << 23), up16 = up * 0.0625f;
   const float back = __int_as_float((127 + 10 + e) << 23) * scale;           // 2^24 / up
+  float start[NG > 4 ? 2 : 1] = {};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     float sum = 0.f;
@@ -132,27 +142,36 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint16_t* q,
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    sum *= -8.f / 16777216.f;
-    f.start[g][0] = __shfl_sync(0xffffffffu, sum, 8 * c);                    // head 2c: lanes 4 (2c) ..
-    f.start[g][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+    if ((g & 3) == c) start[g >> 2] = sum;                                   // k slots 2c, 2c + 1 belong to group c (and c + 4)
   }
-  f.factor[0] = __shfl_sync(0xffffffffu, back, 8 * c);
-  f.factor[1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
+#pragma unroll
+  for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
+    const float x = start[i] * (-8.f / 256.f);                               // |sum| <= 2^20: at most 2^15
+    const __half hi = __float2half_rn(x);
+    const __half2 both = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+    f.start[i] = *reinterpret_cast<const uint32_t*>(&both);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    f.factor[e] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * e);             // head 2c + e: lanes 4 (2c + e) ..
+    f.factor8[e] = f.factor[e] * (256.f / 16777216.f);
+  }
 }
 
 // Running state of a warp: this lane's part of eight heads.
 template <int NG>
 struct Q4State {
   float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), heads 2c + (reg & 1); odd elements times 16
-  float z[NG][4];               // -8 * sum of the rounded p * value scale, in the units of o
-  float m[2], l[2];             // what is subtracted for heads 2c, 2c + 1 (equal in all lanes r), this lane's sum of p
+  float z[4];                   // row g: -8 * sum of the rounded p * value scale of group g, in the units of o (even elements)
+  float m[2], l[2];             // what is subtracted for heads 2c, 2c + 1 (equal in all lanes r), sum of this lane's p
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[g][0][i] = o[g][1][i] = z[g][i] = 0.f;
+      for (int i = 0; i < 4; ++i) o[g][0][i] = o[g][1][i] = 0.f;
     }
-    m[0] = m[1] = -INFINITY;
+    z[0] = z[1] = z[2] = z[3] = 0.f;
+    m[0] = m[1] = kQ4None;
     l[0] = l[1] = 0.f;
   }
 };
@@ -183,6 +202,19 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
   }
   // ---- scores of tokens r, r + 8 and heads 2c, 2c + 1: s[j][e]
   float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  float base8[4];                                // sum over the groups of key scale * start: rows are tokens again
+  {
+    const uint32_t pick = 0x1010u + 0x2222u * (NG == 2 ? lane & 1 : lane & 3);       // scale of group c, twice
+    const uint32_t a0 = __byte_perm(sc[0][0], sc[0][NG == 2 ? 0 : 1], pick), a1 = __byte_perm(sc[1][0], sc[1][NG == 2 ? 0 : 1], pick);
+    if (NG <= 4) {
+      mma_f16_first(base8, a0, a1, 0u, 0u, f.start[0], 0u);
+    } else {
+      const uint32_t pick2 = 0x1010u + 0x2222u * (NG == 6 ? lane & 1 : lane & 3);    // and of group c + 4
+      constexpr int K2 = NG > 4 ? 2 : 0, K3 = NG == 8 ? 3 : K2;
+      mma_f16_first(base8, a0, a1, __byte_perm(sc[0][K2], sc[0][K3], pick2), __byte_perm(sc[1][K2], sc[1][K3], pick2), f.start[0],
+              f.start[NG > 4 ? 1 : 0]);
+    }
+  }
   {
     uint32_t kw[2 * NG];
 #pragma unroll
@@ -192,9 +224,9 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float d[4] = {f.start[g][0], f.start[g][1], f.start[g][0], f.start[g][1]};
+      float d[4];
       const uint32_t a = kw[g], b = kw[NG + g];
-      mma_f16(d, a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u, f.b[g][0], f.b[g][1]);
+      mma_f16_first(d, a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u, f.b[g][0], f.b[g][1]);
       const uint32_t a8 = a >> 8, b8 = b >> 8;
       mma_f16(d, a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u, f.b[g][2], f.b[g][3]);
 #pragma unroll
@@ -206,65 +238,65 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
       }
     }
   }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j][e] = fmaf(base8[2 * j + e], f.factor8[e], s[j][e] * f.factor[e]);
+  }
   if (live < kQ4Tile) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j) {
+      if (r + 8 * j < live) continue;
+      s[j][0] = s[j][1] = -INFINITY;
 #pragma unroll
-      for (int g = NG / 2; g < NG; ++g) sc[j][g] = r + 8 * j < live ? sc[j][g] : 0u;
+      for (int g = NG / 2; g < NG; ++g) sc[j][g] = 0u;
+    }
   }
   // ---- value scales in fp32, their largest magnitude per token
   float sv[2][NG], reach[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    float top = 5.9604645e-8f;                   // 2^-24: a token whose values are all zero still counts in the sum
+    reach[j] = 5.9604645e-8f;                    // 2^-24: a token whose values are all zero still counts in the sum
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&sc[j][(NG + g) >> 1]));
       sv[j][g] = (g & 1) ? two.y : two.x;
-      top = fmaxf(top, fabsf(sv[j][g]));
-    }
-    reach[j] = log2_fast(top);
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) s[j][e] *= f.factor[e];
-  }
-  if (live < kQ4Tile) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (r + 8 * j >= live) s[j][0] = s[j][1] = -INFINITY;
-  }
-  const float top0 = fmaxf(s[0][0] + reach[0], s[1][0] + reach[1]), top1 = fmaxf(s[0][1] + reach[0], s[1][1] + reach[1]);
-  // m is kQ4Top below the maximum at which it was taken
-  if (__any_sync(0xffffffffu, top0 > st.m[0] + (kQ4Top + kQ4Slack) || top1 > st.m[1] + (kQ4Top + kQ4Slack))) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float top = e ? top1 : top0;
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      const float next = fmaxf(st.m[e], top - kQ4Top);
-      const float corr = st.m[e] == -INFINITY ? 0.f : exp2_fast(st.m[e] - next);
-      st.m[e] = next;
-      st.l[e] *= corr;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        st.z[g][e] *= corr;
-        st.z[g][2 + e] *= corr;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) { st.o[g][t][e] *= corr; st.o[g][t][2 + e] *= corr; }
-      }
+      reach[j] = fmaxf(reach[j], fabsf(sv[j][g]));
     }
   }
   float p[2][2];
+  float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const float base = st.m[e] == -INFINITY ? 0.f : st.m[e];
+  for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) p[j][e] = exp2_fast(s[j][e] - base);
-    st.l[e] += p[0][e] + p[1][e];
+    for (int e = 0; e < 2; ++e) {
+      p[j][e] = exp2_fast(s[j][e] - st.m[e]);
+      top = fmaxf(top, p[j][e] * reach[j]);
+    }
   }
+  if (__any_sync(0xffffffffu, top > kQ4Limit)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float most = fmaxf(s[0][e] + log2_fast(reach[0]), s[1][e] + log2_fast(reach[1]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+      const float next = fmaxf(st.m[e], most - kQ4Top);
+      const float corr = exp2_fast(st.m[e] - next);
+      st.m[e] = next;
+      st.l[e] *= corr;
+      st.z[e] *= corr;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) { st.o[g][t][e] *= corr; st.o[g][t][2 + e] *= corr; }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) p[j][e] = exp2_fast(s[j][e] - next);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) st.l[e] += p[0][e] + p[1][e];
   uint32_t vw[2 * NG];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
@@ -278,7 +310,8 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
     const uint32_t v0 = vw[g], v1 = vw[NG + g], w0 = v0 >> 8, w1 = v1 >> 8;
     mma_f16(st.o[g][0], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, b0, b1);
     mma_f16(st.o[g][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, b0, b1);
-    mma_f16(st.z[g], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);      // -8 and -8 * 16, times 2^-24
+    const uint32_t eight = r == g ? 0x80088008u : 0u;                                  // -8 * 2^-24 in row g
+    mma_f16(st.z, eight, 0u, eight, 0u, b0, b1);
   }
 }
 
@@ -291,18 +324,17 @@ __device__ __forceinline__ int q4_len(const Q4DecodeArgs& a, int row) {
 __device__ __forceinline__ int q4_count(int len) { return (len + kQ4Tile - 1) / kQ4Tile; }
 
 // How the call's tiles are dealt out: unit = (row, slice of at most eight heads of a kv head), units in order, all tiles of all
-// units in one line that is cut into `active` equal ranges. Every block finds its place by a sum over the rows' lengths.
+// units in one line that is cut into equal ranges, one for each warp, so that lengths of any mixture keep every warp busy for
+// the same time. A cut inside a unit of at most kQ4Whole tiles moves to its end: joining the parts of a short unit takes longer
+// than a few more tiles. Every block finds the places of its warps by a sum over the rows' lengths.
 struct Q4Plan {
   long long total;              // tiles of the call
-  int active;                   // workers with a range
-  int units;                    // units of a row
-  int row;                      // row that holds tile `at`, and the tiles before that row
-  long long before;
-  __device__ __forceinline__ long long start(int worker) const { return total * worker / active; }
+  long long per;                // of a warp
+  int units;                    // of a row
 };
 
-// `at` is the worker whose first tile is looked for. All threads of the block take part; shared: 2 * kQ4Warps + 4 words of 8.
-__device__ __forceinline__ Q4Plan q4_plan(const Q4DecodeArgs& a, int worker, long long* shared) {
+__device__ __forceinline__ Q4Plan q4_plan(const Q4DecodeArgs& a, int* rows, long long* before) {
+  __shared__ long long sums[kQ4Warps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int each = (a.rows + kQ4Threads - 1) / kQ4Threads, first = threadIdx.x * each, last = min(a.rows, first + each);
   long long mine = 0;
@@ -313,40 +345,38 @@ __device__ __forceinline__ Q4Plan q4_plan(const Q4DecodeArgs& a, int worker, lon
     const long long up = __shfl_up_sync(0xffffffffu, sum, off);
     if (lane >= off) sum += up;
   }
-  if (lane == 31) shared[warp] = sum;
+  if (lane == 31) sums[warp] = sum;
   __syncthreads();
-  long long before = sum - mine, all = 0;
+  long long ahead = sum - mine, all = 0;
 #pragma unroll
   for (int w = 0; w < kQ4Warps; ++w) {
-    if (w < warp) before += shared[w];
-    all += shared[w];
+    if (w < warp) ahead += sums[w];
+    all += sums[w];
   }
   Q4Plan plan;
   plan.units = a.hkv * a.slices;
   plan.total = all * plan.units;
-  plan.active = (int)min((long long)a.workers, max(1LL, plan.total / kQ4MinTiles));
-  plan.row = 0;
-  plan.before = 0;
-  if (worker < plan.active && plan.total > 0) {
-    const long long at = plan.start(worker);
-    if (at >= before * plan.units && at < (before + mine) * plan.units) {
-      int row = first;
-      for (; row < last; ++row) {
-        const int n = q4_count(q4_len(a, row));
-        if (at < (before + n) * plan.units) break;
-        before += n;
-      }
-      shared[kQ4Warps] = row;
-      shared[kQ4Warps + 1] = before * plan.units;
+  const long long workers = (long long)gridDim.x * kQ4Warps, round = plan.total + workers - 1;
+  plan.per = max((long long)kQ4MinTiles, round >> 32 ? round / workers : (long long)((uint32_t)round / (uint32_t)workers));
+#pragma unroll
+  for (int w = 0; w <= kQ4Warps; ++w) {           // the row that holds the first tile of warp w's range
+    const long long at = ((long long)blockIdx.x * kQ4Warps + w) * plan.per;
+    if (at < ahead * plan.units || at >= (ahead + mine) * plan.units) continue;
+    long long b = ahead;
+    int row = first;
+    for (; row < last; ++row) {
+      const int n = q4_count(q4_len(a, row));
+      if (at < (b + n) * plan.units) break;
+      b += n;
     }
-    __syncthreads();
-    plan.row = (int)shared[kQ4Warps];
-    plan.before = shared[kQ4Warps + 1];
+    rows[w] = row;
+    before[w] = b * plan.units;
   }
+  __syncthreads();
   return plan;
 }
 
-// A place in the line of tiles, relative to the worker's first.
+// A place in the line of tiles, relative to the warp's first.
 struct Q4Cursor {
   int row, unit;                // unit within the row
   int begin, end;               // tiles of the unit
@@ -364,210 +394,237 @@ struct Q4Cursor {
   }
 };
 
-template <int NG> __host__ __device__ constexpr int q4_stages() { return NG <= 4 ? 4 : 3; }
-template <int NG> __host__ __device__ constexpr int q4_smem() {
-  return kQ4Warps * q4_stages<NG>() * 576 * NG + (kQ4Warps * 8 * (NG * 32 + 4) + kQ4Warps * 16) * 4;
-}
+template <int NG> __host__ __device__ constexpr int q4_stages() { return 3; }
+template <int NG> __host__ __device__ constexpr int q4_smem() { return kQ4Warps * q4_stages<NG>() * (576 + 512) * NG; }
 
+// Each warp goes its own way through its range: a ring of shared-memory stages, each a tile and, at the start of a unit, the
+// unit's query rows, filled by asynchronous copies that run ahead across units. A unit that lies within the range is finished
+// from registers; parts of others go to `part` for the kernel below.
 template <int NG, bool BF16>
 __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
-  constexpr int HD = NG * 32, TILE = 576 * NG, STAGES = q4_stages<NG>(), REC = HD + 4;
+  constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = TILE + 512 * NG, STAGES = q4_stages<NG>(), REC = HD + 4;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ long long plan_words[kQ4Warps + 2];
-  float* sm_o = reinterpret_cast<float*>(smem + kQ4Warps * STAGES * TILE);          // [warp][8][HD + 4]
-  float* sm_m = sm_o + kQ4Warps * 8 * REC;                                          // [warp][8]
-  float* sm_l = sm_m + kQ4Warps * 8;
+  __shared__ int plan_rows[kQ4Warps + 1];
+  __shared__ long long plan_before[kQ4Warps + 1];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hkv;
+  const int worker = blockIdx.x * kQ4Warps + warp;
   // rows without tokens
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
     if (q4_len(a, row) > 0) continue;
     for (int i = threadIdx.x * 4; i < a.hq * HD; i += kQ4Threads * 4)
       q4_store4<BF16>(a.out + (size_t)row * a.out_stride + i, 0.f, 0.f, 0.f, 0.f);
   }
-  const Q4Plan plan = q4_plan(a, blockIdx.x, plan_words);
-  if (plan.total == 0 || (int)blockIdx.x >= plan.active) return;
-  const long long lo = plan.start(blockIdx.x);
-  const int count = (int)(plan.start(blockIdx.x + 1) - lo);
+  const Q4Plan plan = q4_plan(a, plan_rows, plan_before);
+  // ---- this warp's range
   Q4Cursor now;
-  now.row = plan.row;
-  now.len = q4_len(a, now.row);
+  long long start;
+  int count;
   {
-    const int n = q4_count(now.len);
-    const long long into = lo - plan.before;
-    now.unit = (int)(into / n);
-    now.begin = -(int)(into - (long long)now.unit * n);
-    now.end = now.begin + n;
+    long long at[2];
+#pragma unroll
+    for (int i = 1; i >= 0; --i) {
+      at[i] = min(plan.total, (worker + i) * plan.per);
+      if (at[i] == plan.total) continue;
+      const int row = plan_rows[warp + i], len = q4_len(a, row), n = q4_count(len);
+      const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]), unit = into / (uint32_t)n, off = into - unit * n;
+      now.row = row;
+      now.unit = unit;
+      now.len = len;
+      now.begin = -(int)off;
+      now.end = now.begin + n;
+      if (off > 0 && n <= kQ4Whole) {
+        at[i] += n - off;
+        now.end = 0;
+        now.next(a, plan.units);
+      }
+    }
+    start = at[0];
+    count = (int)(at[1] - at[0]);
   }
-  // ---- copies: each warp takes every fourth tile of the range and keeps STAGES - 1 of them on the way
-  uint8_t* ring = smem + warp * STAGES * TILE;
-  Q4Cursor ahead = now;
-  int fetch = warp, stage_in = 0;
-  uint32_t missing = 0;                          // stages whose page is not in the pool
-  int block = -1, inside = 0;
-  auto locate = [&]() {                          // page of tile `fetch`
-    while (fetch >= ahead.end && fetch < count) ahead.next(a, plan.units);
-    if (fetch < count) {
-      const int t = fetch - ahead.begin;
-      const int page = a.tiles == 1 ? t : (int)__umulhi((uint32_t)t, a.tiles_inverse);
-      inside = t - page * a.tiles;
+  int4 owner = make_int4(-1, 0, 0, 0);
+  if (count > 0) {
+    uint8_t* ring = smem + warp * STAGES * STAGE;
+    const uint32_t to0 = smem_u32(ring) + lane * 16;
+    const uint32_t head_bytes = a.tiles * TILE, page_bytes = a.hkv * head_bytes;
+    Q4Cursor ahead = now;
+    const int* page = nullptr;                   // table entry of tile `fetch`
+    const uint8_t* base = nullptr;               // kv head of `ahead` in page 0, at this lane's piece
+    uint32_t inside = 0;                         // byte of the tile in its page
+    int fetch = 0, stage_in = 0, block = 0;
+    uint32_t missing = 0;                        // stages whose page is not in the pool
+    bool fresh = true;                           // tile `fetch` is the warp's first of its unit
+    auto enter = [&](int t) {
       const int seq = a.seqs != nullptr ? a.seqs[ahead.row] : ahead.row;
-      block = a.block_table[(size_t)seq * a.max_blocks + page];
-    }
-  };
-  auto issue = [&]() {
-    if (fetch < count) {
-      const bool ok = block >= 0 && block < a.num_blocks;
-      missing = ok ? missing & ~(1u << stage_in) : missing | (1u << stage_in);
-      if (ok) {
-        const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices;
-        const uint8_t* from = a.pool + (((size_t)block * a.hkv + kvh) * a.tiles + inside) * TILE + lane * 16;
-        uint8_t* to = ring + stage_in * TILE + lane * 16;
-#pragma unroll
-        for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
-        if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
+      page = a.block_table + (size_t)seq * a.max_blocks;
+      inside = 0;
+      if (t > 0) {
+        const int skip = t / a.tiles;
+        page += skip;
+        inside = (t - skip * a.tiles) * TILE;
       }
-      fetch += kQ4Warps;
-      locate();
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
-  };
-  locate();
+      base = a.pool + (size_t)(a.slices == 1 ? ahead.unit : ahead.unit / a.slices) * head_bytes + lane * 16;
+      block = *page;
+    };
+    auto issue = [&]() {
+      if (fetch < count) {
+        const uint32_t to = to0 + stage_in * STAGE;
+        if ((uint32_t)block < (uint32_t)a.num_blocks) {
+          const uint8_t* from = base + ((size_t)(uint32_t)block * page_bytes + inside);
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue();
+          for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
+          if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
+        } else {
+          missing |= 1u << stage_in;
+        }
+        if (fresh) {
+          const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices, g0 = (ahead.unit - kvh * a.slices) * 8;
+          const int pieces = min(8, group - g0) * (HD / 8);
+          const uint16_t* q = a.q + (size_t)ahead.row * a.q_stride + (size_t)(kvh * group + g0) * HD;
+          for (int i = lane; i < pieces; i += 32) copy16(to + TILE + (i - lane) * 16, q + i * 8);
+          fresh = false;
+        }
+        if (++fetch < count) {
+          if (fetch == ahead.end) {
+            ahead.next(a, plan.units);
+            enter(0);
+            fresh = true;
+          } else {
+            inside += TILE;
+            if (inside == head_bytes) {
+              inside = 0;
+              block = *++page;
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    };
+    enter(-ahead.begin);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue();
 
-  Q4Query<NG> f;
-  Q4State<NG> st;
-  int mine = warp, stage = 0;
-  for (;;) {
-    const int kvh = now.unit / a.slices, g0 = (now.unit - kvh * a.slices) * 8;
-    const int heads = min(8, group - g0), head0 = kvh * group + g0;
-    q4_load_query<NG, BF16>(f, a.q + (size_t)now.row * a.q_stride + (size_t)head0 * HD, heads, a.scale);
-    st.clear();
-    const int stop = min(now.end, count);
-    for (; mine < stop; mine += kQ4Warps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-      __syncwarp();                              // all lanes' pieces have landed; the previous stage has been read
-      const bool gone = missing >> stage & 1;
-      issue();
-      if (!gone) q4_tile<NG>(st, f, ring + stage * TILE, now.len - (mine - now.begin) * kQ4Tile);
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-    }
-    // ---- the warps meet: factors and sums first
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int off = 4; off <= 16; off <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], off);
-      if (st.l[e] != st.l[e] && st.m[e] == -INFINITY) st.m[e] = 0.f;         // NaN scores only: not to be taken for no tokens
-    }
-    __syncthreads();                             // the previous unit's records have been read
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (r == 0) { sm_m[warp * 8 + 2 * c + e] = st.m[e]; sm_l[warp * 8 + 2 * c + e] = st.l[e]; }
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-        *reinterpret_cast<float4*>(sm_o + (warp * 8 + 2 * c + e) * REC + 32 * g + 4 * r) =
-            make_float4((st.o[g][0][e] + st.z[g][e]) * 16777216.f, (st.o[g][0][2 + e] + st.z[g][2 + e]) * 1048576.f,
-                        (st.o[g][1][e] + st.z[g][e]) * 16777216.f, (st.o[g][1][2 + e] + st.z[g][2 + e]) * 1048576.f);
-    }
-    __syncthreads();
-    const bool whole = now.begin >= 0 && now.end <= count;
-    for (int i = threadIdx.x; i < heads * (HD / 4); i += kQ4Threads) {
-      const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kQ4Warps; ++w) top = fmaxf(top, sm_m[w * 8 + h]);
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kQ4Warps; ++w) {
-        const float m = sm_m[w * 8 + h];
-        if (m == -INFINITY) continue;
-        const float x = exp2_fast(m - top);
-        const float4 o = *reinterpret_cast<const float4*>(sm_o + (w * 8 + h) * REC + d);
-        sum += sm_l[w * 8 + h] * x;
-        acc.x += o.x * x; acc.y += o.y * x; acc.z += o.z * x; acc.w += o.w * x;
+    Q4Query<NG> f;
+    Q4State<NG> st;
+    int mine = 0, stage = 0;
+    for (;;) {
+      const int kvh = a.slices == 1 ? now.unit : now.unit / a.slices, g0 = (now.unit - kvh * a.slices) * 8;
+      const int heads = min(8, group - g0), head0 = kvh * group + g0;
+      st.clear();
+      const int stop = min(now.end, count);
+      for (bool first = true; mine < stop; ++mine, first = false) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();                            // all lanes' pieces have landed; the previous stage has been read
+        const uint8_t* tile = ring + stage * STAGE;
+        if (first) q4_load_query<NG, BF16>(f, tile + TILE, heads, a.scale);
+        issue();
+        if (missing >> stage & 1) missing &= ~(1u << stage);
+        else q4_tile<NG>(st, f, tile, now.len - (mine - now.begin) * kQ4Tile);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
-      if (whole) {
-        const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-        q4_store4<BF16>(a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + d, acc.x * inv, acc.y * inv,
-                        acc.z * inv, acc.w * inv);
-      } else {
+      // ---- the unit, or the warp's part of it
+      const bool begins = now.begin >= 0, ends = now.end <= count;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], off);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = 2 * c + e;
+        const bool whole = begins && ends;
         // slot 0: the unit began before this range; slot 1: it goes on after it
-        float* rec = a.part + (((size_t)blockIdx.x * 2 + (now.begin < 0 ? 0 : 1)) * 8 + h) * REC;
-        *reinterpret_cast<float4*>(rec + d) = acc;
-        if (d == 0) { rec[HD] = top; rec[HD + 1] = sum; }
+        float* rec = a.part + (((size_t)worker * 2 + (begins ? 1 : 0)) * a.heads + h) * REC;
+        const float by = !whole ? 16777216.f : st.l[e] == 0.f ? 0.f : 16777216.f / st.l[e];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
+          const float4 o = make_float4((st.o[g][0][e] + z) * by, fmaf(st.o[g][0][2 + e], 0.0625f, z) * by,
+                                       (st.o[g][1][e] + z) * by, fmaf(st.o[g][1][2 + e], 0.0625f, z) * by);
+          if (h >= heads) continue;
+          if (whole) q4_store4<BF16>(a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + 32 * g + 4 * r, o.x, o.y, o.z, o.w);
+          else *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) = o;
+        }
+        if (!whole && h < heads && r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
       }
+      if (begins && !ends) owner = make_int4(now.row, now.unit, (int)((start + now.end - 1) / plan.per), 0);
+      if (now.end >= count) break;
+      now.next(a, plan.units);
     }
-    if (now.end >= count) break;
-    now.next(a, plan.units);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (lane == 0) a.owner[worker] = owner;
 }
+// Joins the parts of units that several warps share: slot 1 of the warp that began it, slot 0 of the others. Block x looks after
+// four workers' units. SPREAD: few long units; block (x, y) does head y, its groups of HD / 4 threads take turns with the records
+// and meet in shared memory. Otherwise a group of threads does all records of a unit's head by itself.
+constexpr int kQ4MergeThreads = 256;
 
-// Units that several workers share. Grid (worker, head of the slice): block (w, h) joins the unit in whose inside worker w
-// starts, if no earlier worker starts inside it too. Records: slot 1 of the worker that began it, slot 0 of the others.
-template <int NG, bool BF16>
-__global__ void __launch_bounds__(kQ4Threads) paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a) {
-  constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4Threads / LANES;
-  __shared__ long long plan_words[kQ4Warps + 2];
-  __shared__ __align__(16) float sm_o[SETS][HD];
+template <int NG, bool BF16, bool SPREAD>
+__global__ void __launch_bounds__(kQ4MergeThreads) paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a) {
+  constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4MergeThreads / LANES;
+  __shared__ __align__(16) float sm_o[SPREAD ? SETS : 1][HD];
   __shared__ float sm_m[SETS], sm_l[SETS];
-  const int worker = blockIdx.x + 1, h = blockIdx.y;
-  const Q4Plan plan = q4_plan(a, worker, plan_words);
+  const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4, group = a.hq / a.hkv;
   // every block waits, also one without work: what follows this kernel follows the attention kernel too
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (plan.total == 0 || worker >= plan.active) return;
-  const int n = q4_count(q4_len(a, plan.row));
-  const long long at = plan.start(worker), into = at - plan.before;
-  const int unit = (int)(into / n);
-  const long long begin = plan.before + (long long)unit * n, end = begin + n;
-  if (begin == at || plan.start(worker - 1) > begin) return;
-  const int kvh = unit / a.slices, g0 = (unit - kvh * a.slices) * 8, group = a.hq / a.hkv;
-  if (h >= min(8, group - g0)) return;
-  // sets of HD / 4 threads take every SETS-th record
-  const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4;
-  float top = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (set < SETS) {
-    for (int w = worker - 1 + set; w < plan.active && plan.start(w) < end; w += SETS) {
-      const float* rec = a.part + (((size_t)w * 2 + (w < worker ? 1 : 0)) * 8 + h) * REC;
-      const float m = rec[HD], l = rec[HD + 1];
-      const float4 o = *reinterpret_cast<const float4*>(rec + d);
-      if (m == -INFINITY) continue;
-      const float next = fmaxf(top, m), x = top == -INFINITY ? 0.f : exp2_fast(top - next), y = exp2_fast(m - next);
-      sum = sum * x + l * y;
-      acc.x = acc.x * x + o.x * y; acc.y = acc.y * x + o.y * y; acc.z = acc.z * x + o.z * y; acc.w = acc.w * x + o.w * y;
-      top = next;
-    }
-    *reinterpret_cast<float4*>(&sm_o[set][d]) = acc;
-    if (d == 0) { sm_m[set] = top; sm_l[set] = sum; }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x * 4; e < HD; e += kQ4Threads * 4) {
-    float all = -INFINITY, total = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  int4 owners[kQ4Warps];
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) all = fmaxf(all, sm_m[s]);
+  for (int i = 0; i < kQ4Warps; ++i) owners[i] = a.owner[blockIdx.x * kQ4Warps + i];
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) {
-      if (sm_m[s] == -INFINITY) continue;
-      const float x = exp2_fast(sm_m[s] - all);
-      const float4 v = *reinterpret_cast<const float4*>(&sm_o[s][e]);
-      total += sm_l[s] * x;
-      o.x += v.x * x; o.y += v.y * x; o.z += v.z * x; o.w += v.w * x;
+  for (int i = 0; i < kQ4Warps; ++i) {
+    if (owners[i].x < 0) continue;
+    const int row = owners[i].x, unit = owners[i].y, last = owners[i].z, worker = blockIdx.x * kQ4Warps + i;
+    const int kvh = unit / a.slices, g0 = (unit - kvh * a.slices) * 8, heads = min(8, group - g0);
+    const int step = SPREAD ? (int)gridDim.y : SETS;
+    for (int h = SPREAD ? blockIdx.y : set < SETS ? set : heads; h < heads; h += step) {
+      float top = kQ4None, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (set < SETS) {
+#pragma unroll 4
+        for (int w = worker + (SPREAD ? set : 0); w <= last; w += SPREAD ? SETS : 1) {
+          const float* rec = a.part + (((size_t)w * 2 + (w == worker ? 1 : 0)) * a.heads + h) * REC;
+          const float2 ml = *reinterpret_cast<const float2*>(rec + HD);
+          const float4 o = *reinterpret_cast<const float4*>(rec + d);
+          const float next = fmaxf(top, ml.x), x = exp2_fast(top - next), y = exp2_fast(ml.x - next);
+          sum = sum * x + ml.y * y;
+          acc.x = acc.x * x + o.x * y; acc.y = acc.y * x + o.y * y; acc.z = acc.z * x + o.z * y; acc.w = acc.w * x + o.w * y;
+          top = next;
+        }
+      }
+      if (SPREAD) {
+        __syncthreads();
+        if (set < SETS) {
+          *reinterpret_cast<float4*>(&sm_o[set][d]) = acc;
+          if (d == 0) { sm_m[set] = top; sm_l[set] = sum; }
+        }
+        __syncthreads();
+        if (set > 0) continue;
+        float all = kQ4None;
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) all = fmaxf(all, sm_m[s]);
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+          const float x = exp2_fast(sm_m[s] - all);
+          const float4 v = *reinterpret_cast<const float4*>(&sm_o[s][d]);
+          sum += sm_l[s] * x;
+          acc.x += v.x * x; acc.y += v.y * x; acc.z += v.z * x; acc.w += v.w * x;
+        }
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      q4_store4<BF16>(a.out + (size_t)row * a.out_stride + (size_t)(kvh * group + g0 + h) * HD + d, acc.x * inv, acc.y * inv,
+                      acc.z * inv, acc.w * inv);
     }
-    const float inv = all == -INFINITY ? 0.f : 1.f / total;
-    q4_store4<BF16>(a.out + (size_t)plan.row * a.out_stride + (size_t)(kvh * group + g0 + h) * HD + e, o.x * inv, o.y * inv,
-                    o.z * inv, o.w * inv);
   }
 }
 
-// Blocks of the attention kernel that the GPU holds at a time: the most workers of a call.
+// Blocks of the attention kernel that the GPU holds at a time: the most of a call.
 template <int NG, bool BF16>
-static int q4_workers() {
+static int q4_blocks() {
   static int known[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -584,25 +641,23 @@ static int q4_workers() {
 }
 
 template <int NG, bool BF16>
-static int launch_q4_decode(Q4DecodeArgs& a, int workers, cudaStream_t st) {
-  const int most = q4_workers<NG, BF16>();
-  if (most < 1) return -5;
-  a.workers = min(workers, most);
-  paged_decode_q4_kernel<NG, BF16><<<a.workers, kQ4Threads, q4_smem<NG>(), st>>>(a);
-  if (a.workers > 1) {
-    // starts while the attention kernel runs, finds its units, waits for the records
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.workers - 1, min(8, a.hq / a.hkv));
-    cfg.blockDim = dim3(kQ4Threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16>, (const Q4DecodeArgs)a);
-    if (e != cudaSuccess) return -(int)e;
-  }
+static int launch_q4_decode(const Q4DecodeArgs& a, int blocks, cudaStream_t st) {
+  if (blocks > q4_blocks<NG, BF16>()) return -5;
+  paged_decode_q4_kernel<NG, BF16><<<blocks, kQ4Threads, q4_smem<NG>(), st>>>(a);
+  // starts while the attention kernel runs out
+  const bool spread = (long long)a.rows * a.hkv * a.slices * 8 < (long long)blocks * kQ4Warps;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, spread ? a.heads : 1);
+  cfg.blockDim = dim3(kQ4MergeThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = spread ? cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, true>, a)
+                               : cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, false>, a);
+  if (e != cudaSuccess) return -(int)e;
   return check_launch("paged_decode_q4");
 }
 
@@ -610,39 +665,44 @@ static int launch_q4_decode(Q4DecodeArgs& a, int workers, cudaStream_t st) {
 
 using namespace icb;
 
-// The most workers of icb_paged_decode_q4 for a head size; negative: not covered.
-ICB_API int icb_paged_decode_q4_workers(int hd, int dtype) {
+// The most blocks of icb_paged_decode_q4 for a head size; negative: not covered.
+ICB_API int icb_paged_decode_q4_blocks(int hd, int dtype) {
   const bool bf = dtype == kBF16;
   switch (hd) {
-    case 64: return bf ? q4_workers<2, true>() : q4_workers<2, false>();
-    case 128: return bf ? q4_workers<4, true>() : q4_workers<4, false>();
-    case 192: return bf ? q4_workers<6, true>() : q4_workers<6, false>();
-    case 256: return bf ? q4_workers<8, true>() : q4_workers<8, false>();
+    case 64: return bf ? q4_blocks<2, true>() : q4_blocks<2, false>();
+    case 128: return bf ? q4_blocks<4, true>() : q4_blocks<4, false>();
+    case 192: return bf ? q4_blocks<6, true>() : q4_blocks<6, false>();
+    case 256: return bf ? q4_blocks<8, true>() : q4_blocks<8, false>();
   }
   return -3;
 }
 
 // q: [rows, hq * hd] 16-bit rows of pitch q_stride (16-byte aligned); pool: num_blocks pages of [hkv][tiles] tiles; row i
 // attends over the first lens[i] tokens of table row seqs[i] (null: i). out: [rows, out_stride], same type. hd 64, 128, 192
-// or 256. scratch: workers * 16 * (hd + 4) floats.
+// or 256. scratch: blocks * 4 * (4 + 2 * min(8, hq / hkv) * (hd + 4)) floats, 16-byte aligned.
 ICB_API int icb_paged_decode_q4(const void* q, long long q_stride, const void* pool, const int* block_table, const int* seqs,
                                 const int* lens, void* out, long long out_stride, void* scratch, int rows, int hq, int hkv,
-                                int hd, int tiles, int max_blocks, int table_rows, int num_blocks, int workers, float scale,
+                                int hd, int tiles, int max_blocks, int table_rows, int num_blocks, int blocks, float scale,
                                 int dtype, void* stream) {
   if (rows <= 0) return 0;
-  if (hkv < 1 || hq < 1 || hq % hkv || tiles < 1 || workers < 1 || q_stride % 8 || (long long)max_blocks * tiles > (1LL << 26)) return -2;
+  if (hkv < 1 || hq < 1 || hq % hkv || tiles < 1 || blocks < 1 || q_stride % 8) return -2;
+  const int slices = (hq / hkv + 7) / 8;
+  // offsets within a page and within a row's units are 32-bit
+  if ((long long)hkv * tiles * 18 * hd > 0x7fffffffLL || (long long)max_blocks * tiles * hkv * slices > 0x7fffffffLL ||
+      (long long)max_blocks * tiles > 0x7ffffffLL)
+    return -2;
   Q4DecodeArgs a{reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<const uint8_t*>(pool), block_table, seqs,
-                 lens, reinterpret_cast<uint16_t*>(out), out_stride, reinterpret_cast<float*>(scratch), rows, hq, hkv,
-                 (hq / hkv + 7) / 8, tiles, max_blocks, table_rows, num_blocks, workers,
-                 (uint32_t)(((1ULL << 32) + tiles - 1) / tiles), scale * kLog2e};
+                 lens, reinterpret_cast<uint16_t*>(out), out_stride, reinterpret_cast<int4*>(scratch),
+                 reinterpret_cast<float*>(scratch) + (size_t)blocks * kQ4Warps * 4, rows, hq, hkv, slices,
+                 hq / hkv < 8 ? hq / hkv : 8, tiles, max_blocks, table_rows, num_blocks, scale * kLog2e};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = dtype == kBF16;
   if (!bf && dtype != kF16) return -4;
   switch (hd) {
-    case 64: return bf ? launch_q4_decode<2, true>(a, workers, st) : launch_q4_decode<2, false>(a, workers, st);
-    case 128: return bf ? launch_q4_decode<4, true>(a, workers, st) : launch_q4_decode<4, false>(a, workers, st);
-    case 192: return bf ? launch_q4_decode<6, true>(a, workers, st) : launch_q4_decode<6, false>(a, workers, st);
-    case 256: return bf ? launch_q4_decode<8, true>(a, workers, st) : launch_q4_decode<8, false>(a, workers, st);
+    case 64: return bf ? launch_q4_decode<2, true>(a, blocks, st) : launch_q4_decode<2, false>(a, blocks, st);
+    case 128: return bf ? launch_q4_decode<4, true>(a, blocks, st) : launch_q4_decode<4, false>(a, blocks, st);
+    case 192: return bf ? launch_q4_decode<6, true>(a, blocks, st) : launch_q4_decode<6, false>(a, blocks, st);
+    case 256: return bf ? launch_q4_decode<8, true>(a, blocks, st) : launch_q4_decode<8, false>(a, blocks, st);
   }
   return -3;
 }

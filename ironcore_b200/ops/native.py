@@ -181,8 +181,18 @@ def ptr(t):
     return t.data_ptr()
 
 
+try:
+    # one call instead of building a Stream object: a few microseconds of every launch
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:  # pragma: no cover - a build of torch without CUDA
+    _raw_stream = None
+
+
 def stream_ptr():
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_current_device())
 
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}

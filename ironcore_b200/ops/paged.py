@@ -7,7 +7,6 @@ holds keys and values; every 32 neighbouring elements of a token's head share an
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import List, Optional, Sequence, Tuple, Union
@@ -23,7 +22,7 @@ native.register("icb_paged_decode", [P, L, P, P, P, P, P, P, I, I, I, I, I, I, F
 native.register("icb_kv_append_q4", [P, P, P, P, L, I, I, I, L, L, L, I, P])
 native.register("icb_kv_read_q4", [P, P, P, P, L, I, I, I, L, I, P])
 native.register("icb_paged_decode_q4", [P, L, P, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, P])
-native.register("icb_paged_decode_q4_workers", [I, I])
+native.register("icb_paged_decode_q4_blocks", [I, I])
 native.register("icb_copy_pages", [P, I, P, P, I, P])
 _SMS = None
 _HALF = (torch.bfloat16, torch.float16)
@@ -113,9 +112,22 @@ def paged_decode(q: torch.Tensor, k_cache, v_cache, block_table, seq_lens, hq: i
 
 
 # --------------------------------------------------------------------------- pages
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
 def _on(t: torch.Tensor):
     """Launches go to the tensor's device, whichever is current."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _page_numbers(x, name: str) -> torch.Tensor:
@@ -191,15 +203,16 @@ def q4_pool_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int
 
 def _q4_sizes(pool: torch.Tensor) -> Tuple[int, int, int, int]:
     """(blocks, kv heads, tiles of a page, head size) of a pool."""
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or pool.shape[3] % 18 or pool.shape[3] // 18 not in Q4_HEAD_DIMS \
-            or pool.shape[1] < 1 or pool.shape[2] < 1:
-        raise ValueError(f"not a 4-bit pool: {pool.dtype} {tuple(pool.shape)}")
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 4 or shape[3] % 18 or shape[3] // 18 not in Q4_HEAD_DIMS or shape[1] < 1 \
+            or shape[2] < 1:
+        raise ValueError(f"not a 4-bit pool: {pool.dtype} {tuple(shape)}")
     if not pool.is_contiguous():
         raise ValueError("a 4-bit pool must be contiguous")
-    return pool.shape[0], pool.shape[1], pool.shape[2], pool.shape[3] // 18
+    return shape[0], shape[1], shape[2], shape[3] // 18
 
 
-def _same_device(pool: torch.Tensor, **others) -> None:
+def _elsewhere(pool: torch.Tensor, **others) -> None:
     for name, t in others.items():
         if t is not None and t.device != pool.device:
             raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
@@ -211,11 +224,11 @@ def _rows16(x: torch.Tensor) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=16)
-def _q4_workers(hd: int, dtype: torch.dtype) -> int:
+def _q4_blocks(hd: int, dtype: torch.dtype) -> int:
     """Blocks of the attention kernel that the GPU holds at a time."""
-    n = native.query("icb_paged_decode_q4_workers", hd, dtype_code(dtype))
+    n = native.query("icb_paged_decode_q4_blocks", hd, dtype_code(dtype))
     if n < 1:
-        raise RuntimeError(f"icb_paged_decode_q4_workers failed with code {n}")
+        raise RuntimeError(f"icb_paged_decode_q4_blocks failed with code {n}")
     return n
 
 
@@ -301,8 +314,10 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slots: to
         raise ValueError(f"rows of {hkv} heads of {hd} expected, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     if slots.dtype != torch.int64 or slots.shape != k.shape[:1]:
         raise ValueError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
-    _same_device(pool, k=k, v=v, slots=slots)
-    if k.is_cuda and k.dtype in _HALF:
+    dev = pool.get_device()
+    if k.get_device() != dev or v.get_device() != dev or slots.get_device() != dev:
+        _elsewhere(pool, k=k, v=v, slots=slots)
+    if dev >= 0 and k.dtype in _HALF:
         with _on(pool):
             k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
             call("icb_kv_append_q4", ptr(k), ptr(v), ptr(pool), ptr(slots), k.shape[0], hkv, hd, tiles, blocks * tiles * 16,
@@ -319,11 +334,14 @@ def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = tor
         raise ValueError(f"slots must be int64 [T], got {slots.dtype} {tuple(slots.shape)}")
     if not dtype.is_floating_point:
         raise ValueError(f"cannot read a cache as {dtype}")
-    _same_device(pool, slots=slots)
-    if pool.is_cuda and dtype in _HALF:
-        t = slots.numel()
+    dev = pool.get_device()
+    if slots.get_device() != dev:
+        _elsewhere(pool, slots=slots)
+    if dev >= 0 and dtype in _HALF:
+        t = slots.shape[0]
         with _on(pool):
-            k, v = torch.empty((2, t, hkv * hd), dtype=dtype, device=pool.device)
+            k = pool.new_empty((t, hkv * hd), dtype=dtype)
+            v = torch.empty_like(k)
             slots = slots.contiguous()
             call("icb_kv_read_q4", ptr(pool), ptr(slots), ptr(k), ptr(v), t, hkv, hd, tiles, blocks * tiles * 16,
                  dtype_code(dtype), stream_ptr())
@@ -336,35 +354,41 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, hq * hd] (row view, any pitch): row i against the first ``seq_lens[i]`` tokens of the sequence whose pages are
     row ``seqs[i]`` of ``block_table`` (int32; None: row i) -> [T, hq * hd], into ``out`` (rows of any pitch) if given.
-    A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens."""
+    A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens. A NaN
+    among the keys or values of a sequence makes the heads that read it NaN."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
-    t = q.shape[0]
-    scale = float(scale) if scale is not None else hd ** -0.5
     if hq < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads do not share {hkv} key / value heads evenly")
     if q.dim() != 2 or q.shape[1] != hq * hd:
         raise ValueError(f"query rows of {hq} heads of {hd} expected, got {tuple(q.shape)}")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
-            or seq_lens.shape != (t,) or (seqs is not None and (seqs.dtype != torch.int32 or seqs.shape != (t,))):
+    t, dtype, i32 = q.shape[0], q.dtype, torch.int32
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if block_table.dim() != 2 or block_table.dtype != i32 or seq_lens.dtype != i32 or seq_lens.shape != (t,) \
+            or (seqs is not None and (seqs.dtype != i32 or seqs.shape != (t,))):
         raise ValueError("block_table [S, pages], seq_lens [T] and seqs [T] must be int32")
-    if seqs is None and block_table.shape[0] < t:
-        raise ValueError(f"{t} rows for {block_table.shape[0]} rows of pages")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(1) != 1):
+    table_rows, pages = block_table.shape
+    if seqs is None and table_rows < t:
+        raise ValueError(f"{t} rows for {table_rows} rows of pages")
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.stride(1) != 1):
         raise ValueError("out must have q's shape and type and neighbouring elements")
-    _same_device(pool, q=q, block_table=block_table, seq_lens=seq_lens, seqs=seqs, out=out)
-    if q.is_cuda and q.dtype in _HALF:
+    dev = pool.get_device()
+    if q.get_device() != dev or block_table.get_device() != dev or seq_lens.get_device() != dev \
+            or (seqs is not None and seqs.get_device() != dev) or (out is not None and out.get_device() != dev):
+        _elsewhere(pool, q=q, block_table=block_table, seq_lens=seq_lens, seqs=seqs, out=out)
+    if dev >= 0 and dtype in _HALF:
         with _on(pool):
             if out is None:
-                out = torch.empty((t, hq * hd), dtype=q.dtype, device=q.device)
+                out = q.new_empty((t, hq * hd))
             q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
-            seqs = seqs.contiguous() if seqs is not None else None
-            # at most a worker for every four tiles of 16 tokens that the table has room for
-            most = t * block_table.shape[1] * tiles * hkv * ((hq // hkv + 7) // 8)
-            workers = max(1, min(_q4_workers(hd, q.dtype), most // 4))
-            scratch = torch.empty(workers * 16 * (hd + 4), dtype=torch.float32, device=q.device)
-            call("icb_paged_decode_q4", ptr(q), q.stride(0), ptr(pool), ptr(block_table), ptr(seqs), ptr(seq_lens), ptr(out),
-                 out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, block_table.shape[1], block_table.shape[0], blocks, workers,
-                 scale, dtype_code(q.dtype), stream_ptr())
+            if seqs is not None:
+                seqs = seqs.contiguous()
+            # four warps to a block, two tiles of 16 tokens at least to a warp: no more than the table has room for
+            per = hq // hkv
+            grid = max(1, min(_q4_blocks(hd, dtype), -(-t * pages * tiles * hkv * ((per + 7) // 8) // 8)))
+            scratch = q.new_empty(grid * (16 + 8 * min(8, per) * (hd + 4)), dtype=torch.float32)
+            call("icb_paged_decode_q4", q.data_ptr(), q.stride(0), pool.data_ptr(), block_table.data_ptr(), ptr(seqs),
+                 seq_lens.data_ptr(), out.data_ptr(), out.stride(0), scratch.data_ptr(), t, hq, hkv, hd, tiles, pages,
+                 table_rows, blocks, grid, scale, dtype_code(dtype), stream_ptr())
         return out
     res = paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs)
     return res if out is None else out.copy_(res)
