@@ -42,7 +42,8 @@ struct Q4DecodeArgs {
   const int* lens;
   uint16_t* out;                // [rows, out_stride], heads HD apart
   long long out_stride;
-  int4* owner;                  // [workers]: {row, unit, last worker} of a unit that begins in a worker's range and goes on
+  int4* owner;                  // {row, unit, first, last worker} of a unit that several warps share, or row -1; one entry for
+  int by_unit;                  // each unit of the call, or (by_unit 0) for each warp: the unit that begins in its range
   float* part;                  // [workers][2][slice heads] records of HD + 4 floats: outputs, maximum, sum
   int rows, hq, hkv, slices, heads, tiles, max_blocks, table_rows, num_blocks;   // heads: of a slice, at most eight
   float scale;                  // score factor times log2(e)
@@ -95,24 +96,25 @@ __device__ __forceinline__ void q4_store4(uint16_t* to, float x, float y, float 
   }
 }
 
-// The query operand of up to eight heads, resident in registers.
+// The query operand, resident in registers: column n of the matrix instructions is head n (T = 1, up to eight heads) or head
+// n & 3 (T = 2, up to four: columns 4 .. 7 are the same heads for a second tile).
 template <int NG>
 struct Q4Query {
   uint32_t b[NG][4];            // B fragments of the two matrix instructions of a group
-  uint32_t start[NG > 4 ? 2 : 1];   // B fragment of -8 * sum of a group's query elements: fp16 and what it leaves
-  float factor[2], factor8[2];  // from the dot products, and from the sums of `start`, to the base-2 score; heads 2c, 2c + 1
+  float start[NG][2];           // -8 * sum of the group's elements, in the units of the dot products (2^-24); columns 2c, 2c + 1
+  float factor[2];              // from the dot products to the base-2 score
 };
 
-template <int NG, bool BF16>
+template <int NG, int T, bool BF16>
 __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, int heads, float scale) {
   constexpr int HD = NG * 32;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = T == 1 ? r : r & 3;
   float x[NG][8];
   float top = 0.f;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (r < heads) u = *reinterpret_cast<const uint4*>(q + (r * HD + g * 32 + c * 8) * 2);
+    if (head < heads) u = *reinterpret_cast<const uint4*>(q + (head * HD + g * 32 + c * 8) * 2);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -127,7 +129,6 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, 
   const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 116);
   const float up = __int_as_float((127 + 14 - e) << 23), up16 = up * 0.0625f;
   const float back = __int_as_float((127 + 10 + e) << 23) * scale;           // 2^24 / up
-  float start[NG > 4 ? 2 : 1] = {};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     float sum = 0.f;
@@ -142,28 +143,20 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, 
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if ((g & 3) == c) start[g >> 2] = sum;                                   // k slots 2c, 2c + 1 belong to group c (and c + 4)
+    sum *= -8.f / 16777216.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f.start[g][i] = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * i);   // column 2c + i: lanes 4 (2c + i) ..
   }
 #pragma unroll
-  for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
-    const float x = start[i] * (-8.f / 256.f);                               // |sum| <= 2^20: at most 2^15
-    const __half hi = __float2half_rn(x);
-    const __half2 both = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
-    f.start[i] = *reinterpret_cast<const uint32_t*>(&both);
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    f.factor[e] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * e);             // head 2c + e: lanes 4 (2c + e) ..
-    f.factor8[e] = f.factor[e] * (256.f / 16777216.f);
-  }
+  for (int i = 0; i < 2; ++i) f.factor[i] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * i);
 }
 
-// Running state of a warp: this lane's part of eight heads.
+// Running state of a warp: this lane's part of eight columns.
 template <int NG>
 struct Q4State {
-  float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), heads 2c + (reg & 1); odd elements times 16
+  float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), columns 2c + (reg & 1); odd elements times 16
   float z[4];                   // row g: -8 * sum of the rounded p * value scale of group g, in the units of o (even elements)
-  float m[2], l[2];             // what is subtracted for heads 2c, 2c + 1 (equal in all lanes r), sum of this lane's p
+  float m[2], l[2];             // what is subtracted in columns 2c, 2c + 1 (equal in all lanes r), sum of this lane's p
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -174,18 +167,48 @@ struct Q4State {
     m[0] = m[1] = kQ4None;
     l[0] = l[1] = 0.f;
   }
+  __device__ __forceinline__ void rescale(int e, float by) {
+    l[e] *= by;
+    z[e] *= by;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) { o[g][t][e] *= by; o[g][t][2 + e] *= by; }
+    }
+  }
+  // Columns n and n + 4 hold the same head over different tokens: both become their sum.
+  __device__ __forceinline__ void fold() {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float other = __shfl_xor_sync(0xffffffffu, m[e], 2), next = fmaxf(m[e], other);
+      rescale(e, exp2_fast(m[e] - next));
+      m[e] = next;
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      z[e] += __shfl_xor_sync(0xffffffffu, z[e], 2);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          o[g][t][e] += __shfl_xor_sync(0xffffffffu, o[g][t][e], 2);
+          o[g][t][2 + e] += __shfl_xor_sync(0xffffffffu, o[g][t][2 + e], 2);
+        }
+      }
+    }
+  }
 };
 
-// One tile of 16 tokens in shared memory; `live` of them belong to the sequence (16 or more: all).
-template <int NG>
-__device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, const uint8_t* tile, int live) {
-  constexpr int NP = NG / 2;                     // 16-byte pieces per lane of the keys, and of the values
-  const int lane = threadIdx.x & 31, r = lane >> 2;
-  // scales of tokens r and r + 8: NG fp16 of the keys, NG of the values
+// T tiles of 16 tokens in shared memory, neighbours in the sequence; `live` tokens belong to the sequence (16 T or more: all),
+// bit j of `gone`: tile T - 1 - j is not there. With T = 2 both tiles go through the same columns' arithmetic at once: columns
+// 0 .. 3 are the heads over the first tile, 4 .. 7 over the second, which a group of at most four heads would leave idle.
+template <int NG, int T>
+__device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG>& f, const uint8_t* tiles, int live, uint32_t gone) {
+  constexpr int NP = NG / 2, TILE = 576 * NG;    // NP: 16-byte pieces per lane of the keys, and of the values
+  const int lane = threadIdx.x & 31, r = lane >> 2, second = T == 2 ? (lane >> 1) & 1 : 0;
+  // scales of tokens r and r + 8 of this lane's tile: NG fp16 of the keys, NG of the values
   uint32_t sc[2][NG];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const uint8_t* at = tile + 512 * NG + (r + 8 * j) * 4 * NG;
+    const uint8_t* at = tiles + second * TILE + 512 * NG + (r + 8 * j) * 4 * NG;
     if (NG % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < NG / 4; ++i) {
@@ -200,54 +223,46 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
       }
     }
   }
-  // ---- scores of tokens r, r + 8 and heads 2c, 2c + 1: s[j][e]
-  float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  float base8[4];                                // sum over the groups of key scale * start: rows are tokens again
+  // ---- scores of tokens r, r + 8 and columns 2c, 2c + 1: s[2 j + e]
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   {
-    const uint32_t pick = 0x1010u + 0x2222u * (NG == 2 ? lane & 1 : lane & 3);       // scale of group c, twice
-    const uint32_t a0 = __byte_perm(sc[0][0], sc[0][NG == 2 ? 0 : 1], pick), a1 = __byte_perm(sc[1][0], sc[1][NG == 2 ? 0 : 1], pick);
-    if (NG <= 4) {
-      mma_f16_first(base8, a0, a1, 0u, 0u, f.start[0], 0u);
-    } else {
-      const uint32_t pick2 = 0x1010u + 0x2222u * (NG == 6 ? lane & 1 : lane & 3);    // and of group c + 4
-      constexpr int K2 = NG > 4 ? 2 : 0, K3 = NG == 8 ? 3 : K2;
-      mma_f16_first(base8, a0, a1, __byte_perm(sc[0][K2], sc[0][K3], pick2), __byte_perm(sc[1][K2], sc[1][K3], pick2), f.start[0],
-              f.start[NG > 4 ? 1 : 0]);
-    }
-  }
-  {
-    uint32_t kw[2 * NG];
+    uint32_t kw[T][2 * NG];
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const uint4 u = *reinterpret_cast<const uint4*>(tile + p * 512 + lane * 16);
-      kw[4 * p] = u.x; kw[4 * p + 1] = u.y; kw[4 * p + 2] = u.z; kw[4 * p + 3] = u.w;
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const uint4 u = *reinterpret_cast<const uint4*>(tiles + t * TILE + p * 512 + lane * 16);
+        kw[t][4 * p] = u.x; kw[t][4 * p + 1] = u.y; kw[t][4 * p + 2] = u.z; kw[t][4 * p + 3] = u.w;
+      }
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float d[4];
-      const uint32_t a = kw[g], b = kw[NG + g];
-      mma_f16_first(d, a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u, f.b[g][0], f.b[g][1]);
-      const uint32_t a8 = a >> 8, b8 = b >> 8;
-      mma_f16(d, a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u, f.b[g][2], f.b[g][3]);
+      float d[T][4];
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const uint32_t a = kw[t][g], b = kw[t][NG + g], a8 = a >> 8, b8 = b >> 8;
+        mma_f16_first(d[t], a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u, f.b[g][0], f.b[g][1]);
+        mma_f16(d[t], a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u, f.b[g][2], f.b[g][3]);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&sc[j][g >> 1]));
         const float ks = (g & 1) ? two.y : two.x;
-        s[j][0] = fmaf(ks, d[2 * j], s[j][0]);
-        s[j][1] = fmaf(ks, d[2 * j + 1], s[j][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float dot = T == 2 && second ? d[T - 1][2 * j + e] : d[0][2 * j + e];
+          s[2 * j + e] = fmaf(ks, dot + f.start[g][e], s[2 * j + e]);
+        }
       }
     }
   }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) s[j][e] = fmaf(base8[2 * j + e], f.factor8[e], s[j][e] * f.factor[e]);
-  }
-  if (live < kQ4Tile) {
+  if (live < T * kQ4Tile || gone != 0u) {
+    asm volatile("" ::: "memory");               // a branch: nearly all passes skip it
+    const int mine = (gone >> (T - 1 - second) & 1) ? 0 : live - second * kQ4Tile;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if (r + 8 * j < live) continue;
-      s[j][0] = s[j][1] = -INFINITY;
+      if (r + 8 * j < mine) continue;
+      s[2 * j] = s[2 * j + 1] = -INFINITY;
 #pragma unroll
       for (int g = NG / 2; g < NG; ++g) sc[j][g] = 0u;
     }
@@ -264,54 +279,53 @@ __device__ __forceinline__ void q4_tile(Q4State<NG>& st, const Q4Query<NG>& f, c
       reach[j] = fmaxf(reach[j], fabsf(sv[j][g]));
     }
   }
-  float p[2][2];
+  float p[4];
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      p[j][e] = exp2_fast(s[j][e] - st.m[e]);
-      top = fmaxf(top, p[j][e] * reach[j]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    p[i] = exp2_fast(fmaf(s[i], f.factor[i & 1], -st.m[i & 1]));
+    top = fmaxf(top, p[i] * reach[i >> 1]);
   }
   if (__any_sync(0xffffffffu, top > kQ4Limit)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float most = fmaxf(s[0][e] + log2_fast(reach[0]), s[1][e] + log2_fast(reach[1]));
+      float most = fmaxf(fmaf(s[e], f.factor[e], log2_fast(reach[0])), fmaf(s[2 + e], f.factor[e], log2_fast(reach[1])));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
       const float next = fmaxf(st.m[e], most - kQ4Top);
-      const float corr = exp2_fast(st.m[e] - next);
+      st.rescale(e, exp2_fast(st.m[e] - next));
       st.m[e] = next;
-      st.l[e] *= corr;
-      st.z[e] *= corr;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) { st.o[g][t][e] *= corr; st.o[g][t][2 + e] *= corr; }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) p[j][e] = exp2_fast(s[j][e] - next);
+      p[e] = exp2_fast(fmaf(s[e], f.factor[e], -next));
+      p[2 + e] = exp2_fast(fmaf(s[2 + e], f.factor[e], -next));
     }
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e) st.l[e] += p[0][e] + p[1][e];
-  uint32_t vw[2 * NG];
+  for (int e = 0; e < 2; ++e) st.l[e] += p[e] + p[2 + e];
+  // ---- V^T P^T
+  uint32_t vw[T][2 * NG];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const uint4 u = *reinterpret_cast<const uint4*>(tile + 256 * NG + i * 512 + lane * 16);
-    vw[4 * i] = u.x; vw[4 * i + 1] = u.y; vw[4 * i + 2] = u.z; vw[4 * i + 3] = u.w;
+  for (int t = 0; t < T; ++t) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const uint4 u = *reinterpret_cast<const uint4*>(tiles + t * TILE + 256 * NG + i * 512 + lane * 16);
+      vw[t][4 * i] = u.x; vw[t][4 * i + 1] = u.y; vw[t][4 * i + 2] = u.z; vw[t][4 * i + 3] = u.w;
+    }
   }
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const uint32_t b0 = transpose8(pack_f16x2(p[0][0] * sv[0][g], p[0][1] * sv[0][g]));
-    const uint32_t b1 = transpose8(pack_f16x2(p[1][0] * sv[1][g], p[1][1] * sv[1][g]));
-    const uint32_t v0 = vw[g], v1 = vw[NG + g], w0 = v0 >> 8, w1 = v1 >> 8;
-    mma_f16(st.o[g][0], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, b0, b1);
-    mma_f16(st.o[g][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, b0, b1);
+    const uint32_t b0 = transpose8(pack_f16x2(p[0] * sv[0][g], p[1] * sv[0][g]));
+    const uint32_t b1 = transpose8(pack_f16x2(p[2] * sv[1][g], p[3] * sv[1][g]));
     const uint32_t eight = r == g ? 0x80088008u : 0u;                                  // -8 * 2^-24 in row g
     mma_f16(st.z, eight, 0u, eight, 0u, b0, b1);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const uint32_t mine = T == 1 ? 0xffffffffu : (r >> 2) == t ? 0xffffffffu : 0u;   // the columns of this tile
+      const uint32_t x0 = b0 & mine, x1 = b1 & mine;
+      const uint32_t v0 = vw[t][g], v1 = vw[t][NG + g], w0 = v0 >> 8, w1 = v1 >> 8;
+      mma_f16(st.o[g][0], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, x0, x1);
+      mma_f16(st.o[g][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, x0, x1);
+    }
   }
 }
 
@@ -394,15 +408,17 @@ struct Q4Cursor {
   }
 };
 
-template <int NG> __host__ __device__ constexpr int q4_stages() { return 3; }
-template <int NG> __host__ __device__ constexpr int q4_smem() { return kQ4Warps * q4_stages<NG>() * (576 + 512) * NG; }
+template <int NG, int T> __host__ __device__ constexpr int q4_stage() { return 576 * NG * T + 512 * NG / T; }
+template <int NG, int T> __host__ __device__ constexpr int q4_stages() { return T == 1 ? 3 : 2; }
+template <int NG, int T> __host__ __device__ constexpr int q4_smem() { return kQ4Warps * q4_stages<NG, T>() * q4_stage<NG, T>(); }
 
-// Each warp goes its own way through its range: a ring of shared-memory stages, each a tile and, at the start of a unit, the
+// Each warp goes its own way through its range: a ring of shared-memory stages, each T tiles and, at the start of a unit, the
 // unit's query rows, filled by asynchronous copies that run ahead across units. A unit that lies within the range is finished
 // from registers; parts of others go to `part` for the kernel below.
-template <int NG, bool BF16>
+template <int NG, int T, bool BF16>
 __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
-  constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = TILE + 512 * NG, STAGES = q4_stages<NG>(), REC = HD + 4;
+  constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = q4_stage<NG, T>(), STAGES = q4_stages<NG, T>(), REC = HD + 4;
+  constexpr int COLUMNS = 8 / T;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int plan_rows[kQ4Warps + 1];
   __shared__ long long plan_before[kQ4Warps + 1];
@@ -410,12 +426,6 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hkv;
   const int worker = blockIdx.x * kQ4Warps + warp;
-  // rows without tokens
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (q4_len(a, row) > 0) continue;
-    for (int i = threadIdx.x * 4; i < a.hq * HD; i += kQ4Threads * 4)
-      q4_store4<BF16>(a.out + (size_t)row * a.out_stride + i, 0.f, 0.f, 0.f, 0.f);
-  }
   const Q4Plan plan = q4_plan(a, plan_rows, plan_before);
   // ---- this warp's range
   Q4Cursor now;
@@ -447,94 +457,90 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
   if (count > 0) {
     uint8_t* ring = smem + warp * STAGES * STAGE;
     const uint32_t to0 = smem_u32(ring) + lane * 16;
-    const uint32_t head_bytes = a.tiles * TILE, page_bytes = a.hkv * head_bytes;
+    const uint8_t* from0 = a.pool + lane * 16;
+    // Tiles to come, 32 at a time: lane i looks up the place of the i-th (its number among the pool's tiles; -1: not in the
+    // pool, or behind the range), all in one unit.
     Q4Cursor ahead = now;
-    const int* page = nullptr;                   // table entry of tile `fetch`
-    const uint8_t* base = nullptr;               // kv head of `ahead` in page 0, at this lane's piece
-    uint32_t inside = 0;                         // byte of the tile in its page
-    int fetch = 0, stage_in = 0, block = 0;
-    uint32_t missing = 0;                        // stages whose page is not in the pool
-    bool fresh = true;                           // tile `fetch` is the warp's first of its unit
-    auto enter = [&](int t) {
-      const int seq = a.seqs != nullptr ? a.seqs[ahead.row] : ahead.row;
-      page = a.block_table + (size_t)seq * a.max_blocks;
-      inside = 0;
-      if (t > 0) {
-        const int skip = t / a.tiles;
-        page += skip;
-        inside = (t - skip * a.tiles) * TILE;
+    int fetched = 0, list = -1, at = 0, filled = 0;        // tiles listed so far, this lane's, next one of the list, its length
+    bool entered = false;                                  // the unit that `ahead` is in has been begun
+    uint32_t stage_in = 0, missing = 0;                    // bits: tiles that are not there, the last one issued lowest
+    auto refill = [&]() {
+      at = 0;
+      filled = 32;
+      list = -1;
+      if (fetched >= count) return;
+      if (fetched == ahead.end) {
+        ahead.next(a, plan.units);
+        entered = false;
       }
-      base = a.pool + (size_t)(a.slices == 1 ? ahead.unit : ahead.unit / a.slices) * head_bytes + lane * 16;
-      block = *page;
+      const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices;
+      if (!entered) {                                      // the unit's query rows travel with its first tile
+        const int g0 = (ahead.unit - kvh * a.slices) * 8, pieces = min(COLUMNS, group - g0) * (HD / 8);
+        const uint16_t* q = a.q + (size_t)ahead.row * a.q_stride + (size_t)(kvh * group + g0) * HD;
+        for (int i = lane; i < pieces; i += 32) copy16(to0 + stage_in + T * TILE + (i - lane) * 16, q + i * 8);
+        entered = true;
+      }
+      filled = min(32, min(ahead.end, count) - fetched);
+      if (lane < filled) {
+        const int seq = a.seqs != nullptr ? a.seqs[ahead.row] : ahead.row;
+        const int t = fetched + lane - ahead.begin, page = a.tiles == 1 ? t : t / a.tiles;
+        const int block = a.block_table[(size_t)seq * a.max_blocks + page];
+        if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + (t - page * a.tiles);
+      }
+      fetched += filled;
     };
     auto issue = [&]() {
-      if (fetch < count) {
-        const uint32_t to = to0 + stage_in * STAGE;
-        if ((uint32_t)block < (uint32_t)a.num_blocks) {
-          const uint8_t* from = base + ((size_t)(uint32_t)block * page_bytes + inside);
+      if (at >= filled) refill();
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int tile = __shfl_sync(0xffffffffu, list, at + t);
+        missing = missing * 2 + (tile < 0);
+        if (tile >= 0) {
+          const uint8_t* from = from0 + (size_t)(uint32_t)tile * TILE;
+          const uint32_t to = to0 + stage_in + t * TILE;
 #pragma unroll
           for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
           if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
-        } else {
-          missing |= 1u << stage_in;
-        }
-        if (fresh) {
-          const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices, g0 = (ahead.unit - kvh * a.slices) * 8;
-          const int pieces = min(8, group - g0) * (HD / 8);
-          const uint16_t* q = a.q + (size_t)ahead.row * a.q_stride + (size_t)(kvh * group + g0) * HD;
-          for (int i = lane; i < pieces; i += 32) copy16(to + TILE + (i - lane) * 16, q + i * 8);
-          fresh = false;
-        }
-        if (++fetch < count) {
-          if (fetch == ahead.end) {
-            ahead.next(a, plan.units);
-            enter(0);
-            fresh = true;
-          } else {
-            inside += TILE;
-            if (inside == head_bytes) {
-              inside = 0;
-              block = *++page;
-            }
-          }
         }
       }
+      at += T;
       asm volatile("cp.async.commit_group;" ::: "memory");
-      stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+      stage_in = stage_in == (STAGES - 1) * STAGE ? 0 : stage_in + STAGE;
     };
-    enter(-ahead.begin);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) issue();
 
     Q4Query<NG> f;
     Q4State<NG> st;
-    int mine = 0, stage = 0;
+    int mine = 0;
+    const uint8_t* tiles = ring;
     for (;;) {
       const int kvh = a.slices == 1 ? now.unit : now.unit / a.slices, g0 = (now.unit - kvh * a.slices) * 8;
-      const int heads = min(8, group - g0), head0 = kvh * group + g0;
+      const int heads = min(COLUMNS, group - g0), head0 = kvh * group + g0;
       st.clear();
       const int stop = min(now.end, count);
-      for (bool first = true; mine < stop; ++mine, first = false) {
+      int live = now.len - (mine - now.begin) * kQ4Tile;
+      for (bool first = true; mine < stop; mine += T, live -= T * kQ4Tile, first = false) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                            // all lanes' pieces have landed; the previous stage has been read
-        const uint8_t* tile = ring + stage * STAGE;
-        if (first) q4_load_query<NG, BF16>(f, tile + TILE, heads, a.scale);
+        const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
+        if (first) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
         issue();
-        if (missing >> stage & 1) missing &= ~(1u << stage);
-        else q4_tile<NG>(st, f, tile, now.len - (mine - now.begin) * kQ4Tile);
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        q4_pass<NG, T>(st, f, tiles, live, gone);
+        tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
       }
+      mine = stop;
       // ---- the unit, or the warp's part of it
-      const bool begins = now.begin >= 0, ends = now.end <= count;
+      const bool begins = now.begin >= 0, ends = now.end <= count, whole = begins && ends;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], off);
       }
+      if (T == 2) st.fold();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = 2 * c + e;
-        const bool whole = begins && ends;
         // slot 0: the unit began before this range; slot 1: it goes on after it
         float* rec = a.part + (((size_t)worker * 2 + (begins ? 1 : 0)) * a.heads + h) * REC;
         const float by = !whole ? 16777216.f : st.l[e] == 0.f ? 0.f : 16777216.f / st.l[e];
@@ -549,81 +555,208 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
         }
         if (!whole && h < heads && r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
       }
-      if (begins && !ends) owner = make_int4(now.row, now.unit, (int)((start + now.end - 1) / plan.per), 0);
+      if (begins) {
+        owner = whole ? make_int4(-1, 0, 0, 0) : make_int4(now.row, now.unit, worker, (int)((start + now.end - 1) / plan.per));
+        if (a.by_unit && lane == 0) a.owner[(size_t)now.row * plan.units + now.unit] = owner;
+      }
       if (now.end >= count) break;
       now.next(a, plan.units);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  if (lane == 0) a.owner[worker] = owner;
-}
-// Joins the parts of units that several warps share: slot 1 of the warp that began it, slot 0 of the others. Block x looks after
-// four workers' units. SPREAD: few long units; block (x, y) does head y, its groups of HD / 4 threads take turns with the records
-// and meet in shared memory. Otherwise a group of threads does all records of a unit's head by itself.
-constexpr int kQ4MergeThreads = 256;
-
-template <int NG, bool BF16, bool SPREAD>
-__global__ void __launch_bounds__(kQ4MergeThreads) paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a) {
-  constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4MergeThreads / LANES;
-  __shared__ __align__(16) float sm_o[SPREAD ? SETS : 1][HD];
-  __shared__ float sm_m[SETS], sm_l[SETS];
-  const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4, group = a.hq / a.hkv;
-  // every block waits, also one without work: what follows this kernel follows the attention kernel too
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int4 owners[kQ4Warps];
-#pragma unroll
-  for (int i = 0; i < kQ4Warps; ++i) owners[i] = a.owner[blockIdx.x * kQ4Warps + i];
-#pragma unroll
-  for (int i = 0; i < kQ4Warps; ++i) {
-    if (owners[i].x < 0) continue;
-    const int row = owners[i].x, unit = owners[i].y, last = owners[i].z, worker = blockIdx.x * kQ4Warps + i;
-    const int kvh = unit / a.slices, g0 = (unit - kvh * a.slices) * 8, heads = min(8, group - g0);
-    const int step = SPREAD ? (int)gridDim.y : SETS;
-    for (int h = SPREAD ? blockIdx.y : set < SETS ? set : heads; h < heads; h += step) {
-      float top = kQ4None, sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (set < SETS) {
-#pragma unroll 4
-        for (int w = worker + (SPREAD ? set : 0); w <= last; w += SPREAD ? SETS : 1) {
-          const float* rec = a.part + (((size_t)w * 2 + (w == worker ? 1 : 0)) * a.heads + h) * REC;
-          const float2 ml = *reinterpret_cast<const float2*>(rec + HD);
-          const float4 o = *reinterpret_cast<const float4*>(rec + d);
-          const float next = fmaxf(top, ml.x), x = exp2_fast(top - next), y = exp2_fast(ml.x - next);
-          sum = sum * x + ml.y * y;
-          acc.x = acc.x * x + o.x * y; acc.y = acc.y * x + o.y * y; acc.z = acc.z * x + o.z * y; acc.w = acc.w * x + o.w * y;
-          top = next;
-        }
-      }
-      if (SPREAD) {
-        __syncthreads();
-        if (set < SETS) {
-          *reinterpret_cast<float4*>(&sm_o[set][d]) = acc;
-          if (d == 0) { sm_m[set] = top; sm_l[set] = sum; }
-        }
-        __syncthreads();
-        if (set > 0) continue;
-        float all = kQ4None;
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) all = fmaxf(all, sm_m[s]);
-        sum = 0.f;
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-          const float x = exp2_fast(sm_m[s] - all);
-          const float4 v = *reinterpret_cast<const float4*>(&sm_o[s][d]);
-          sum += sm_l[s] * x;
-          acc.x += v.x * x; acc.y += v.y * x; acc.z += v.z * x; acc.w += v.w * x;
-        }
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      q4_store4<BF16>(a.out + (size_t)row * a.out_stride + (size_t)(kvh * group + g0 + h) * HD + d, acc.x * inv, acc.y * inv,
-                      acc.z * inv, acc.w * inv);
-    }
+  if (!a.by_unit && lane == 0) a.owner[worker] = owner;
+  // rows without tokens
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (q4_len(a, row) > 0) continue;
+    for (int i = threadIdx.x * 4; i < a.hq * HD; i += kQ4Threads * 4)
+      q4_store4<BF16>(a.out + (size_t)row * a.out_stride + i, 0.f, 0.f, 0.f, 0.f);
+    if (a.by_unit)
+      for (int u = threadIdx.x; u < plan.units; u += kQ4Threads) a.owner[(size_t)row * plan.units + u] = make_int4(-1, 0, 0, 0);
   }
 }
 
+// A block for each unit, whose warps take turns with its tiles and meet in shared memory: one launch, nothing to plan, two
+// dependent loads before the first tile. For tables so narrow that the longest unit keeps its warps busy only shortly.
+template <int NG, int T, bool BF16>
+__global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kernel(const __grid_constant__ Q4DecodeArgs a) {
+  constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = q4_stage<NG, T>(), STAGES = q4_stages<NG, T>(), REC = HD + 4;
+  constexpr int COLUMNS = 8 / T;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warps = blockDim.x >> 5, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int units = a.hkv * a.slices, row = blockIdx.x / units, unit = blockIdx.x - row * units, group = a.hq / a.hkv;
+  const int kvh = a.slices == 1 ? unit : unit / a.slices, g0 = (unit - kvh * a.slices) * 8;
+  const int heads = min(COLUMNS, group - g0), head0 = kvh * group + g0;
+  const int len = q4_len(a, row), n = q4_count(len), passes = (n + T - 1) / T;
+  // passes warp, warp + warps, ... are this warp's; lane i looks up the place of its i-th tile from `listed` on
+  uint8_t* ring = smem + warp * STAGES * STAGE;
+  const uint32_t to0 = smem_u32(ring) + lane * 16;
+  const uint8_t* from0 = a.pool + lane * 16;
+  const int* pages = a.block_table + (size_t)(a.seqs != nullptr ? max(0, min(a.seqs[row], a.table_rows - 1)) : row) * a.max_blocks;
+  int listed = 0, list = -1;
+  auto refill = [&]() {
+    const int i = listed + lane, t = (warp + i / T * warps) * T + i % T;
+    list = -1;
+    if (t < n) {
+      const int page = a.tiles == 1 ? t : t / a.tiles, block = pages[page];
+      if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + (t - page * a.tiles);
+    }
+    listed += 32;
+  };
+  int at = 0;
+  uint32_t stage_in = 0, missing = 0;
+  auto issue = [&]() {
+    if (at == listed) refill();
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int tile = __shfl_sync(0xffffffffu, list, (at + t) & 31);
+      missing = missing * 2 + (tile < 0);
+      if (tile >= 0) {
+        const uint8_t* from = from0 + (size_t)(uint32_t)tile * TILE;
+        const uint32_t to = to0 + stage_in + t * TILE;
+#pragma unroll
+        for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
+        if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
+      }
+    }
+    at += T;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    stage_in = stage_in == (STAGES - 1) * STAGE ? 0 : stage_in + STAGE;
+  };
+  if (warp < passes) {
+    const uint16_t* q = a.q + (size_t)row * a.q_stride + (size_t)head0 * HD;
+    for (int i = lane; i < heads * (HD / 8); i += 32) copy16(to0 + T * TILE + (i - lane) * 16, q + i * 8);
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) issue();
+  }
+  Q4Query<NG> f;
+  Q4State<NG> st;
+  st.clear();
+  const uint8_t* tiles = ring;
+  for (int pass = warp; pass < passes; pass += warps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();                                // all lanes' pieces have landed; the previous stage has been read
+    const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
+    if (pass == warp) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
+    issue();
+    q4_pass<NG, T>(st, f, tiles, len - pass * T * kQ4Tile, gone);
+    tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int off = 4; off <= 16; off <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], off);
+  }
+  __syncthreads();                               // the ring becomes the meeting place: [warp][column] records
+  float* records = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float* rec = records + (warp * 8 + 2 * c + e) * REC;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
+      *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) =
+          make_float4(st.o[g][0][e] + z, fmaf(st.o[g][0][2 + e], 0.0625f, z), st.o[g][1][e] + z, fmaf(st.o[g][1][2 + e], 0.0625f, z));
+    }
+    if (r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
+  }
+  __syncthreads();
+  const int parts = min(warps, passes) * T;      // of a head: column h of each warp, and h + 4 with T = 2
+  for (int i = threadIdx.x; i < heads * (HD / 4); i += blockDim.x) {
+    const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
+    const float* rec = records + h * REC;
+    float top = kQ4None, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, rec[p * COLUMNS * REC + HD]);
+    for (int p = 0; p < parts; ++p) {
+      const float* x = rec + p * COLUMNS * REC;
+      const float by = exp2_fast(x[HD] - top);
+      const float4 o = *reinterpret_cast<const float4*>(x + d);
+      sum += x[HD + 1] * by;
+      acc.x += o.x * by; acc.y += o.y * by; acc.z += o.z * by; acc.w += o.w * by;
+    }
+    const float by = sum == 0.f ? 0.f : 16777216.f / sum;
+    q4_store4<BF16>(a.out + (size_t)row * a.out_stride + (size_t)(head0 + h) * HD + d, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
+  }
+}
+
+// Joins the parts of units that several warps share: slot 1 of the warp that began it, slot 0 of the others. A task is a head of
+// an entry of `owner`. SPREAD: few long units; a block does one task, its groups of HD / 4 threads take turns with the records and
+// meet in shared memory. Otherwise each group of threads does a task by itself.
+constexpr int kQ4MergeThreads = 256;
+
+template <int NG, bool BF16, bool SPREAD>
+__global__ void __launch_bounds__(kQ4MergeThreads) paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long tasks) {
+  constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4MergeThreads / LANES, DEPTH = 8;
+  __shared__ __align__(16) float sm_o[SPREAD ? SETS : 1][HD];
+  __shared__ float sm_m[SETS], sm_l[SETS];
+  const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4, group = a.hq / a.hkv;
+  const long long task = SPREAD ? blockIdx.x : (long long)blockIdx.x * SETS + set;
+  // every block waits, also one without work: what follows this kernel follows the attention kernel too
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (task >= tasks || (!SPREAD && set >= SETS)) return;
+  const long long entry = task / a.heads;
+  const int h = (int)(task - entry * a.heads);
+  const int4 owner = a.owner[entry];
+  if (owner.x < 0) return;
+  const int kvh = owner.y / a.slices, g0 = (owner.y - kvh * a.slices) * 8;
+  if (h >= group - g0) return;
+  float top = kQ4None, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int STEP = SPREAD ? SETS : 1;
+  for (int w0 = owner.z + (SPREAD ? set : 0); w0 <= owner.w && set < SETS; w0 += DEPTH * STEP) {
+    float2 ml[DEPTH];
+    float4 o[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {            // all on the way before the first is used
+      const int w = w0 + i * STEP;
+      ml[i] = make_float2(kQ4None, 0.f);
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (w > owner.w) continue;
+      const float* rec = a.part + (((size_t)w * 2 + (w == owner.z ? 1 : 0)) * a.heads + h) * REC;
+      ml[i] = *reinterpret_cast<const float2*>(rec + HD);
+      o[i] = *reinterpret_cast<const float4*>(rec + d);
+    }
+    float next = top;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) next = fmaxf(next, ml[i].x);
+    const float x = exp2_fast(top - next);
+    sum *= x; acc.x *= x; acc.y *= x; acc.z *= x; acc.w *= x;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const float y = exp2_fast(ml[i].x - next);
+      sum += ml[i].y * y;
+      acc.x += o[i].x * y; acc.y += o[i].y * y; acc.z += o[i].z * y; acc.w += o[i].w * y;
+    }
+    top = next;
+  }
+  if (SPREAD) {
+    if (set < SETS) {
+      *reinterpret_cast<float4*>(&sm_o[set][d]) = acc;
+      if (d == 0) { sm_m[set] = top; sm_l[set] = sum; }
+    }
+    __syncthreads();
+    if (set > 0) return;
+    float all = kQ4None;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) all = fmaxf(all, sm_m[s]);
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      const float x = exp2_fast(sm_m[s] - all);
+      const float4 v = *reinterpret_cast<const float4*>(&sm_o[s][d]);
+      sum += sm_l[s] * x;
+      acc.x += v.x * x; acc.y += v.y * x; acc.z += v.z * x; acc.w += v.w * x;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  q4_store4<BF16>(a.out + (size_t)owner.x * a.out_stride + (size_t)(kvh * group + g0 + h) * HD + d, acc.x * inv, acc.y * inv,
+                  acc.z * inv, acc.w * inv);
+}
+
 // Blocks of the attention kernel that the GPU holds at a time: the most of a call.
-template <int NG, bool BF16>
+template <int NG, int T, bool BF16>
 static int q4_blocks() {
   static int known[64] = {};
   int dev = 0;
@@ -631,23 +764,53 @@ static int q4_blocks() {
   int& n = known[dev];
   if (n == 0) {
     int per_sm = 0;
-    auto k = paged_decode_q4_kernel<NG, BF16>;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_smem<NG>()) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kQ4Threads, q4_smem<NG>()) != cudaSuccess || per_sm < 1)
+    auto k = paged_decode_q4_kernel<NG, T, BF16>;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, q4_smem<NG, T>()) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kQ4Threads, q4_smem<NG, T>()) != cudaSuccess || per_sm < 1)
       return -1;
     n = per_sm * num_sms();
   }
   return n;
 }
 
-template <int NG, bool BF16>
-static int launch_q4_decode(const Q4DecodeArgs& a, int blocks, cudaStream_t st) {
-  if (blocks > q4_blocks<NG, BF16>()) return -5;
-  paged_decode_q4_kernel<NG, BF16><<<blocks, kQ4Threads, q4_smem<NG>(), st>>>(a);
+// Warps of a block of the kernel for whole units; 0: the call goes to the kernel for ranges. Enough of them to fill the GPU with
+// ten warps to an SM, no more than two tiles each need. A warp with more than 32 tiles would hold the others up when the
+// lengths differ: 4 rows of 30000 tokens on 8 kv heads take 104 us here with 16 warps and 45 us in ranges, 512 rows of 768
+// tokens on 2 kv heads 37 us here with 2 warps and 43 us in ranges, 8 rows of 4000 on 32 kv heads 41 us here with 8 and 47 us.
+static int q4_unit_warps(int hd, long long units, long long tiles) {
+  const int most = hd <= 128 ? 16 : 8;
+  int warps = 1;
+  while (warps < most && units * warps < 10LL * num_sms() && tiles > 2 * warps) warps *= 2;
+  return tiles <= 32 * warps && units <= 0x7fffffffLL ? warps : 0;
+}
+
+template <int NG, int T, bool BF16>
+static int launch_q4_units(const Q4DecodeArgs& a, int warps, long long units, cudaStream_t st) {
+  auto k = paged_decode_q4_unit_kernel<NG, T, BF16>;
+  constexpr int ring = q4_stages<NG, T>() * q4_stage<NG, T>(), record = 8 * (NG * 32 + 4) * 4, each = ring > record ? ring : record;
+  static int ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (NG <= 4 ? 16 : 8) * each) != cudaSuccess) return -5;
+    ready[dev] = 1;
+  }
+  k<<<(unsigned)units, warps * 32, warps * each, st>>>(a);
+  return check_launch("paged_decode_q4");
+}
+
+template <int NG, int T, bool BF16>
+static int launch_q4_decode(Q4DecodeArgs& a, int blocks, cudaStream_t st) {
+  if (blocks > q4_blocks<NG, T, BF16>()) return -5;
+  const long long units = (long long)a.rows * a.hkv * a.slices, workers = (long long)blocks * kQ4Warps;
+  a.by_unit = units <= workers;                  // an entry for each unit or each warp, whichever are fewer
+  paged_decode_q4_kernel<NG, T, BF16><<<blocks, kQ4Threads, q4_smem<NG, T>(), st>>>(a);
   // starts while the attention kernel runs out
-  const bool spread = (long long)a.rows * a.hkv * a.slices * 8 < (long long)blocks * kQ4Warps;
+  const bool spread = units * 8 < workers;       // more than eight parts to a unit
+  const long long tasks = (a.by_unit ? units : workers) * a.heads;
+  constexpr int SETS = kQ4MergeThreads / (NG * 8);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks, spread ? a.heads : 1);
+  cfg.gridDim = dim3((unsigned)(spread ? tasks : (tasks + SETS - 1) / SETS));
   cfg.blockDim = dim3(kQ4MergeThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -655,54 +818,62 @@ static int launch_q4_decode(const Q4DecodeArgs& a, int blocks, cudaStream_t st) 
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = spread ? cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, true>, a)
-                               : cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, false>, a);
+  const cudaError_t e = spread ? cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, true>, a, tasks)
+                               : cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, false>, a, tasks);
   if (e != cudaSuccess) return -(int)e;
   return check_launch("paged_decode_q4");
+}
+
+// What a call needs of a variant: blocks of the kernel for ranges that fit the GPU (run false), or the call itself. T = 2 where at most four query heads
+// share a kv head: at 32 heads on 8, T = 1 leaves half of the columns idle.
+template <bool RUN>
+static int q4_variant(int hd, int per, int dtype, Q4DecodeArgs* a, int blocks, int warps, cudaStream_t st) {
+#define ICB_Q4(NG_, T_, BF_) \
+  if (hd == NG_ * 32 && (per > 4 ? 1 : 2) == T_ && dtype == (BF_ ? kBF16 : kF16)) { \
+    if (RUN && warps > 0) return launch_q4_units<NG_, T_, BF_>(*a, warps, (long long)a->rows * a->hkv * a->slices, st); \
+    if (RUN) return launch_q4_decode<NG_, T_, BF_>(*a, blocks, st); \
+    return q4_blocks<NG_, T_, BF_>(); \
+  }
+#define ICB_Q4_TYPES(NG_) ICB_Q4(NG_, 1, true) ICB_Q4(NG_, 2, true) ICB_Q4(NG_, 1, false) ICB_Q4(NG_, 2, false)
+  ICB_Q4_TYPES(2) ICB_Q4_TYPES(4) ICB_Q4_TYPES(6) ICB_Q4_TYPES(8)
+#undef ICB_Q4_TYPES
+#undef ICB_Q4
+  return -3;
 }
 
 }  // namespace icb
 
 using namespace icb;
 
-// The most blocks of icb_paged_decode_q4 for a head size; negative: not covered.
-ICB_API int icb_paged_decode_q4_blocks(int hd, int dtype) {
-  const bool bf = dtype == kBF16;
-  switch (hd) {
-    case 64: return bf ? q4_blocks<2, true>() : q4_blocks<2, false>();
-    case 128: return bf ? q4_blocks<4, true>() : q4_blocks<4, false>();
-    case 192: return bf ? q4_blocks<6, true>() : q4_blocks<6, false>();
-    case 256: return bf ? q4_blocks<8, true>() : q4_blocks<8, false>();
-  }
-  return -3;
+// How icb_paged_decode_q4 is to run a call of `units` = rows * hkv * ceil(hq / hkv / 8) whose table rows hold `tiles` times 16
+// tokens: positive, the `warps` of a block for each unit; negative, minus the `blocks` that share the tiles. 0: not covered.
+ICB_API int icb_paged_decode_q4_plan(int hd, int per, int dtype, long long units, long long tiles) {
+  const int fit = q4_variant<false>(hd, per, dtype, nullptr, 0, 0, nullptr);
+  if (fit < 1) return 0;
+  const int warps = q4_unit_warps(hd, units, tiles);
+  if (warps > 0) return warps;
+  const long long need = (units * tiles + kQ4Warps * kQ4MinTiles - 1) / (kQ4Warps * kQ4MinTiles);
+  return -(int)(need < 1 ? 1 : need < fit ? need : fit);
 }
 
 // q: [rows, hq * hd] 16-bit rows of pitch q_stride (16-byte aligned); pool: num_blocks pages of [hkv][tiles] tiles; row i
 // attends over the first lens[i] tokens of table row seqs[i] (null: i). out: [rows, out_stride], same type. hd 64, 128, 192
-// or 256. scratch: blocks * 4 * (4 + 2 * min(8, hq / hkv) * (hd + 4)) floats, 16-byte aligned.
+// or 256. plan: as icb_paged_decode_q4_plan gives it; where it is negative, scratch has blocks * 4 * (4 + 2 * min(8, hq / hkv)
+// * (hd + 4)) floats, 16-byte aligned.
 ICB_API int icb_paged_decode_q4(const void* q, long long q_stride, const void* pool, const int* block_table, const int* seqs,
                                 const int* lens, void* out, long long out_stride, void* scratch, int rows, int hq, int hkv,
-                                int hd, int tiles, int max_blocks, int table_rows, int num_blocks, int blocks, float scale,
+                                int hd, int tiles, int max_blocks, int table_rows, int num_blocks, int plan, float scale,
                                 int dtype, void* stream) {
   if (rows <= 0) return 0;
-  if (hkv < 1 || hq < 1 || hq % hkv || tiles < 1 || blocks < 1 || q_stride % 8) return -2;
-  const int slices = (hq / hkv + 7) / 8;
-  // offsets within a page and within a row's units are 32-bit
-  if ((long long)hkv * tiles * 18 * hd > 0x7fffffffLL || (long long)max_blocks * tiles * hkv * slices > 0x7fffffffLL ||
-      (long long)max_blocks * tiles > 0x7ffffffLL)
+  if (hkv < 1 || hq < 1 || hq % hkv || tiles < 1 || plan == 0 || plan > (hd <= 128 ? 16 : 8) || q_stride % 8) return -2;
+  const int slices = (hq / hkv + 7) / 8, blocks = plan < 0 ? -plan : 0;
+  // the numbers of a pool's tiles and of a row's tiles in all units are 32-bit
+  if ((long long)max_blocks * tiles * hkv * slices > 0x7fffffffLL || (long long)max_blocks * tiles > 0x7ffffffLL ||
+      (long long)num_blocks * hkv * tiles > 0x7fffffffLL || (long long)rows * hkv * slices > 0x7fffffffLL)
     return -2;
   Q4DecodeArgs a{reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<const uint8_t*>(pool), block_table, seqs,
-                 lens, reinterpret_cast<uint16_t*>(out), out_stride, reinterpret_cast<int4*>(scratch),
+                 lens, reinterpret_cast<uint16_t*>(out), out_stride, reinterpret_cast<int4*>(scratch), 0,
                  reinterpret_cast<float*>(scratch) + (size_t)blocks * kQ4Warps * 4, rows, hq, hkv, slices,
                  hq / hkv < 8 ? hq / hkv : 8, tiles, max_blocks, table_rows, num_blocks, scale * kLog2e};
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf = dtype == kBF16;
-  if (!bf && dtype != kF16) return -4;
-  switch (hd) {
-    case 64: return bf ? launch_q4_decode<2, true>(a, blocks, st) : launch_q4_decode<2, false>(a, blocks, st);
-    case 128: return bf ? launch_q4_decode<4, true>(a, blocks, st) : launch_q4_decode<4, false>(a, blocks, st);
-    case 192: return bf ? launch_q4_decode<6, true>(a, blocks, st) : launch_q4_decode<6, false>(a, blocks, st);
-    case 256: return bf ? launch_q4_decode<8, true>(a, blocks, st) : launch_q4_decode<8, false>(a, blocks, st);
-  }
-  return -3;
+  return q4_variant<true>(hd, hq / hkv, dtype, &a, blocks, plan > 0 ? plan : 0, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -129,9 +129,13 @@ def load(strict: bool = False):
         return _LIB
 
 
+_ENTRIES = {}      # entry points that have been called
+
+
 def register(name: str, argtypes) -> None:
     """Declare one more exported symbol (used by modules that own extra kernels)."""
     _SIGNATURES[name] = argtypes
+    _ENTRIES.pop(name, None)
     if isinstance(_LIB, _UnitLibrary):
         _LIB.__dict__.pop(name, None)
     elif _LIB is not None:
@@ -159,8 +163,9 @@ def reset_launches() -> None:
 def call(name: str, *args) -> int:
     """Invoke an exported function; raise on a non-zero return code."""
     global _LAUNCHES
-    lib = load(strict=True)
-    fn = getattr(lib, name)
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(load(strict=True), name)
     rc = fn(*args)
     _LAUNCHES += 1
     if rc != 0:

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -22,7 +22,7 @@ native.register("icb_paged_decode", [P, L, P, P, P, P, P, P, I, I, I, I, I, I, F
 native.register("icb_kv_append_q4", [P, P, P, P, L, I, I, I, L, L, L, I, P])
 native.register("icb_kv_read_q4", [P, P, P, P, L, I, I, I, L, I, P])
 native.register("icb_paged_decode_q4", [P, L, P, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, P])
-native.register("icb_paged_decode_q4_blocks", [I, I])
+native.register("icb_paged_decode_q4_plan", [I, I, I, L, L])
 native.register("icb_copy_pages", [P, I, P, P, I, P])
 _SMS = None
 _HALF = (torch.bfloat16, torch.float16)
@@ -112,22 +112,9 @@ def paged_decode(q: torch.Tensor, k_cache, v_cache, block_table, seq_lens, hq: i
 
 
 # --------------------------------------------------------------------------- pages
-class _Here:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        pass
-
-
-_HERE = _Here()
-
-
-def _on(t: torch.Tensor):
-    """Launches go to the tensor's device, whichever is current."""
-    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _elsewhere(dev: int) -> bool:
+    """Whether a launch for tensors on CUDA device ``dev`` needs another current device."""
+    return dev >= 0 and dev != torch.cuda.current_device()
 
 
 def _page_numbers(x, name: str) -> torch.Tensor:
@@ -135,7 +122,7 @@ def _page_numbers(x, name: str) -> torch.Tensor:
         if not all(isinstance(n, int) for n in x):
             raise ValueError(f"{name} must be a list of page numbers")
         x = torch.tensor(list(x), dtype=torch.int64)
-    if x.dim() != 1 or x.is_floating_point() or x.dtype == torch.bool:
+    if x.dim() != 1 or x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be a list of page numbers")
     return x
 
@@ -146,50 +133,59 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src, dst) -> 
     twice or be both written and read. ``src``, ``dst`` on the host (lists, CPU tensors) are checked for that and for their
     range; int32 tensors on the device are taken as they are, pairs with a page outside a pool being left out."""
     stacked = isinstance(pools, torch.Tensor)
-    tensors: List[torch.Tensor] = [pools] if stacked else list(pools)
+    tensors: Sequence[torch.Tensor] = (pools,) if stacked else pools
     src, dst = _page_numbers(src, "src"), _page_numbers(dst, "dst")
-    if src.numel() != dst.numel():
-        raise ValueError(f"{src.numel()} source pages for {dst.numel()} destinations")
+    n = src.shape[0]
+    if n != dst.shape[0]:
+        raise ValueError(f"{n} source pages for {dst.shape[0]} destinations")
     if not tensors:
         return
     lead = 1 if stacked else 0
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
+    records = []
     for t in tensors:
         if t.dim() <= lead or not t.is_contiguous():
             raise ValueError("a pool must be contiguous, pages first" + (" after the layers" if stacked else ""))
-        if t.device != dev:
+        if t.get_device() != dev:
             raise ValueError("the pools must be on one device")
-    pages = min(t.shape[lead] for t in tensors)
-    for x, other in ((src, dst), (dst, src)):
-        if x.is_cuda and (x.device != dev or other.device != dev or x.dtype != torch.int32):
+        if t.numel():
+            size, strides = t.element_size(), t.stride()
+            records += (t.data_ptr(), t.shape[0] if stacked else 1, strides[0] * size if stacked else 0, t.shape[lead],
+                        strides[lead] * size)
+    if src.get_device() >= 0 or dst.get_device() >= 0:
+        if not src.get_device() == dst.get_device() == dev or not src.dtype == dst.dtype == torch.int32:
             raise ValueError("page numbers on the device must be int32, both on the pools' device")
-    if not src.is_cuda:
+    else:
+        pages = min(t.shape[lead] for t in tensors)
         a, b = src.tolist(), dst.tolist()
-        if any(not 0 <= n < pages for n in a + b):
+        if any(not 0 <= x < pages for x in a + b):
             raise ValueError(f"page numbers must be in [0, {pages})")
         if len(set(b)) != len(b) or not set(a).isdisjoint(b):
             raise ValueError("a page may be written once, and not be read by another pair")
-    if src.numel() == 0:
+    if n == 0 or not records:
         return
-    if dev.type == "cuda":
-        with _on(tensors[0]):
-            src, dst = (x.to(dev, torch.int32).contiguous() for x in (src, dst))
-            records = []
-            for t in tensors:
-                if t.numel():
-                    size = t.element_size()
-                    records += [t.data_ptr(), t.shape[0] if stacked else 1, t.stride(0) * size if stacked else 0,
-                                t.shape[lead], t.stride(lead) * size]
-            if records:
-                call("icb_copy_pages", (ctypes.c_longlong * len(records))(*records), len(records) // 5, ptr(src), ptr(dst),
-                     src.numel(), stream_ptr())
+    if dev < 0:
+        a, b = src.long(), dst.long()
+        for t in tensors:
+            if stacked:
+                t[:, b] = t[:, a]
+            else:
+                t[b] = t[a]
         return
-    a, b = src.long(), dst.long()
-    for t in tensors:
-        if stacked:
-            t[:, b] = t[:, a]
-        else:
-            t[b] = t[a]
+    if src.get_device() < 0:
+        both = torch.stack((src, dst)).to(tensors[0].device, torch.int32)
+        src, dst = both[0], both[1]
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            copy_pages(pools, src, dst)
+        return
+    src, dst = src.contiguous(), dst.contiguous()
+    call("icb_copy_pages", _records(len(records))(*records), len(records) // 5, src.data_ptr(), dst.data_ptr(), n, stream_ptr())
+
+
+@functools.lru_cache(maxsize=64)
+def _records(n: int):
+    return ctypes.c_longlong * n
 
 
 # --------------------------------------------------------------------------- the 4-bit cache
@@ -201,18 +197,24 @@ def q4_pool_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int
     return num_blocks, kv_heads, block_size // 16, 18 * head_dim
 
 
-def _q4_sizes(pool: torch.Tensor) -> Tuple[int, int, int, int]:
-    """(blocks, kv heads, tiles of a page, head size) of a pool."""
-    shape = pool.shape
-    if pool.dtype != torch.uint8 or len(shape) != 4 or shape[3] % 18 or shape[3] // 18 not in Q4_HEAD_DIMS or shape[1] < 1 \
-            or shape[2] < 1:
-        raise ValueError(f"not a 4-bit pool: {pool.dtype} {tuple(shape)}")
-    if not pool.is_contiguous():
-        raise ValueError("a 4-bit pool must be contiguous")
+@functools.lru_cache(maxsize=64)
+def _q4_shape(shape: torch.Size) -> Optional[Tuple[int, int, int, int]]:
+    if len(shape) != 4 or shape[3] % 18 or shape[3] // 18 not in Q4_HEAD_DIMS or shape[1] < 1 or shape[2] < 1:
+        return None
     return shape[0], shape[1], shape[2], shape[3] // 18
 
 
-def _elsewhere(pool: torch.Tensor, **others) -> None:
+def _q4_sizes(pool: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(blocks, kv heads, tiles of a page, head size) of a pool."""
+    sizes = _q4_shape(pool.shape)
+    if sizes is None or pool.dtype != torch.uint8:
+        raise ValueError(f"not a 4-bit pool: {pool.dtype} {tuple(pool.shape)}")
+    if not pool.is_contiguous() or pool.data_ptr() % 16:
+        raise ValueError("a 4-bit pool must be contiguous and start on a 16-byte boundary")
+    return sizes
+
+
+def _not_together(pool: torch.Tensor, **others) -> None:
     for name, t in others.items():
         if t is not None and t.device != pool.device:
             raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
@@ -220,16 +222,17 @@ def _elsewhere(pool: torch.Tensor, **others) -> None:
 
 def _rows16(x: torch.Tensor) -> torch.Tensor:
     """Rows that 16-byte loads can read: neighbouring elements, aligned starts."""
-    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 else x.contiguous()
+    row, col = x.stride()
+    return x if col == 1 and row % 8 == 0 and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
-@functools.lru_cache(maxsize=16)
-def _q4_blocks(hd: int, dtype: torch.dtype) -> int:
-    """Blocks of the attention kernel that the GPU holds at a time."""
-    n = native.query("icb_paged_decode_q4_blocks", hd, dtype_code(dtype))
-    if n < 1:
-        raise RuntimeError(f"icb_paged_decode_q4_blocks failed with code {n}")
-    return n
+@functools.lru_cache(maxsize=512)
+def _q4_plan(hd: int, per: int, dtype: torch.dtype, units: int, tiles: int) -> Tuple[int, int]:
+    """(how the attention kernel runs a call, floats of scratch memory that it needs)."""
+    plan = native.query("icb_paged_decode_q4_plan", hd, per, dtype_code(dtype), units, tiles)
+    if plan == 0:
+        raise RuntimeError(f"icb_paged_decode_q4 has no kernel for heads of {hd} in {dtype}")
+    return plan, -plan * (16 + 8 * min(8, per) * (hd + 4)) if plan < 0 else 0
 
 
 @functools.lru_cache(maxsize=16)
@@ -310,20 +313,24 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slots: to
     block * block_size + offset; rows with a slot outside the pool are left out). Two rows with one slot: either may win,
     element by element."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
-    if k.dim() != 2 or k.shape != v.shape or k.shape[1] != hkv * hd or k.dtype != v.dtype:
-        raise ValueError(f"rows of {hkv} heads of {hd} expected, got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    if slots.dtype != torch.int64 or slots.shape != k.shape[:1]:
-        raise ValueError(f"slots must be int64 [{k.shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 2 or shape != v.shape or shape[1] != hkv * hd or dtype != v.dtype:
+        raise ValueError(f"rows of {hkv} heads of {hd} expected, got {tuple(shape)} {dtype} and {tuple(v.shape)} {v.dtype}")
+    if slots.dtype != torch.int64 or slots.shape != shape[:1]:
+        raise ValueError(f"slots must be int64 [{shape[0]}], got {slots.dtype} {tuple(slots.shape)}")
     dev = pool.get_device()
-    if k.get_device() != dev or v.get_device() != dev or slots.get_device() != dev:
-        _elsewhere(pool, k=k, v=v, slots=slots)
-    if dev >= 0 and k.dtype in _HALF:
-        with _on(pool):
-            k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
-            call("icb_kv_append_q4", ptr(k), ptr(v), ptr(pool), ptr(slots), k.shape[0], hkv, hd, tiles, blocks * tiles * 16,
-                 k.stride(0), v.stride(0), dtype_code(k.dtype), stream_ptr())
+    if not k.get_device() == v.get_device() == slots.get_device() == dev:
+        _not_together(pool, k=k, v=v, slots=slots)
+    if dev < 0 or dtype not in _HALF:
+        kv_append_q4_reference(k, v, pool, slots)
         return
-    kv_append_q4_reference(k, v, pool, slots)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            kv_append_q4(k, v, pool, slots)
+        return
+    k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
+    call("icb_kv_append_q4", k.data_ptr(), v.data_ptr(), pool.data_ptr(), slots.data_ptr(), shape[0], hkv, hd, tiles,
+         blocks * tiles * 16, k.stride(0), v.stride(0), dtype_code(dtype), stream_ptr())
 
 
 def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
@@ -332,21 +339,23 @@ def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = tor
     blocks, hkv, tiles, hd = _q4_sizes(pool)
     if slots.dtype != torch.int64 or slots.dim() != 1:
         raise ValueError(f"slots must be int64 [T], got {slots.dtype} {tuple(slots.shape)}")
-    if not dtype.is_floating_point:
-        raise ValueError(f"cannot read a cache as {dtype}")
     dev = pool.get_device()
     if slots.get_device() != dev:
-        _elsewhere(pool, slots=slots)
-    if dev >= 0 and dtype in _HALF:
-        t = slots.shape[0]
-        with _on(pool):
-            k = pool.new_empty((t, hkv * hd), dtype=dtype)
-            v = torch.empty_like(k)
-            slots = slots.contiguous()
-            call("icb_kv_read_q4", ptr(pool), ptr(slots), ptr(k), ptr(v), t, hkv, hd, tiles, blocks * tiles * 16,
-                 dtype_code(dtype), stream_ptr())
-        return k, v
-    return kv_read_q4_reference(pool, slots, dtype)
+        _not_together(pool, slots=slots)
+    if dev < 0 or dtype not in _HALF:
+        if not dtype.is_floating_point:
+            raise ValueError(f"cannot read a cache as {dtype}")
+        return kv_read_q4_reference(pool, slots, dtype)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_read_q4(pool, slots, dtype)
+    t = slots.shape[0]
+    k = pool.new_empty((t, hkv * hd), dtype=dtype)
+    v = torch.empty_like(k)
+    slots = slots.contiguous()
+    call("icb_kv_read_q4", pool.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, hkv, hd, tiles,
+         blocks * tiles * 16, dtype_code(dtype), stream_ptr())
+    return k, v
 
 
 def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, hq: int,
@@ -357,38 +366,39 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
     A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens. A NaN
     among the keys or values of a sequence makes the heads that read it NaN."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
+    shape, dtype, i32 = q.shape, q.dtype, torch.int32
     if hq < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads do not share {hkv} key / value heads evenly")
-    if q.dim() != 2 or q.shape[1] != hq * hd:
-        raise ValueError(f"query rows of {hq} heads of {hd} expected, got {tuple(q.shape)}")
-    t, dtype, i32 = q.shape[0], q.dtype, torch.int32
+    if len(shape) != 2 or shape[1] != hq * hd:
+        raise ValueError(f"query rows of {hq} heads of {hd} expected, got {tuple(shape)}")
+    t, rows, per = shape[0], shape[:1], hq // hkv
     scale = hd ** -0.5 if scale is None else float(scale)
-    if block_table.dim() != 2 or block_table.dtype != i32 or seq_lens.dtype != i32 or seq_lens.shape != (t,) \
-            or (seqs is not None and (seqs.dtype != i32 or seqs.shape != (t,))):
+    if block_table.dim() != 2 or block_table.dtype != i32 or seq_lens.dtype != i32 or seq_lens.shape != rows \
+            or (seqs is not None and (seqs.dtype != i32 or seqs.shape != rows)):
         raise ValueError("block_table [S, pages], seq_lens [T] and seqs [T] must be int32")
     table_rows, pages = block_table.shape
     if seqs is None and table_rows < t:
         raise ValueError(f"{t} rows for {table_rows} rows of pages")
-    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.stride(1) != 1):
+    if out is not None and (out.shape != shape or out.dtype != dtype or out.stride(1) != 1):
         raise ValueError("out must have q's shape and type and neighbouring elements")
     dev = pool.get_device()
-    if q.get_device() != dev or block_table.get_device() != dev or seq_lens.get_device() != dev \
+    if not q.get_device() == block_table.get_device() == seq_lens.get_device() == dev \
             or (seqs is not None and seqs.get_device() != dev) or (out is not None and out.get_device() != dev):
-        _elsewhere(pool, q=q, block_table=block_table, seq_lens=seq_lens, seqs=seqs, out=out)
-    if dev >= 0 and dtype in _HALF:
-        with _on(pool):
-            if out is None:
-                out = q.new_empty((t, hq * hd))
-            q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
-            if seqs is not None:
-                seqs = seqs.contiguous()
-            # four warps to a block, two tiles of 16 tokens at least to a warp: no more than the table has room for
-            per = hq // hkv
-            grid = max(1, min(_q4_blocks(hd, dtype), -(-t * pages * tiles * hkv * ((per + 7) // 8) // 8)))
-            scratch = q.new_empty(grid * (16 + 8 * min(8, per) * (hd + 4)), dtype=torch.float32)
-            call("icb_paged_decode_q4", q.data_ptr(), q.stride(0), pool.data_ptr(), block_table.data_ptr(), ptr(seqs),
-                 seq_lens.data_ptr(), out.data_ptr(), out.stride(0), scratch.data_ptr(), t, hq, hkv, hd, tiles, pages,
-                 table_rows, blocks, grid, scale, dtype_code(dtype), stream_ptr())
-        return out
-    res = paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs)
-    return res if out is None else out.copy_(res)
+        _not_together(pool, q=q, block_table=block_table, seq_lens=seq_lens, seqs=seqs, out=out)
+    if dev < 0 or dtype not in _HALF:
+        res = paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs)
+        return res if out is None else out.copy_(res)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_decode_q4(q, pool, block_table, seq_lens, hq, scale, seqs=seqs, out=out)
+    if out is None:
+        out = q.new_empty(shape)
+    q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
+    if seqs is not None:
+        seqs = seqs.contiguous()
+    plan, floats = _q4_plan(hd, per, dtype, t * hkv * ((per + 7) // 8), pages * tiles)
+    scratch = q.new_empty(floats, dtype=torch.float32) if floats else None
+    call("icb_paged_decode_q4", q.data_ptr(), q.stride(0), pool.data_ptr(), block_table.data_ptr(), ptr(seqs),
+         seq_lens.data_ptr(), out.data_ptr(), out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, pages, table_rows, blocks,
+         plan, scale, dtype_code(dtype), stream_ptr())
+    return out
