@@ -5,9 +5,9 @@
 // n = clamp(round(x / scale), -8, 7) + 8, ties to even.
 //
 // Rounding without a division: x and scale have at most 11 significant bits, so x / scale is either a tie k + 1/2 or differs
-// from one by at least 2^-15 of its value, 2^-16 or more. y = x * (1 / scale) with the correctly rounded reciprocal is off by
-// at most 2^-21 (|y| <= 8), and fma(x, 1 / scale, 48) rounds it to a multiple of 2^-18: ties come out as ties, everything else
-// stays on its side of them. Adding 1.5 * 2^23 - 40 then rounds to an integer, ties to even, whose low bits are the code.
+// from one by at least 2^-15 of its value, 2^-16 or more. y = x * (1 / scale) with a reciprocal within 2^-23 is off by at most
+// 2^-20 (|y| <= 8), and fma(x, 1 / scale, 48) rounds it to a multiple of 2^-18: ties come out as ties, everything else stays on
+// its side of them. Adding 1.5 * 2^23 - 40 then rounds to an integer, ties to even, whose low bits are the code.
 //
 // Both directions are bound by memory. Two forms each: one thread per 8 elements of a row, for few rows; and one warp per tile
 // of 16 rows and head in the order of the tile's lanes, so that all 18 hd bytes of the tile leave or arrive in 512-byte pieces
@@ -40,45 +40,61 @@ __device__ __forceinline__ void widen8(const uint4& u, float (&x)[8]) {
   }
 }
 
-// Scale of a group from its extremes; a NaN among the elements makes it NaN.
-__device__ __forceinline__ __half q4_scale(float most, float least) {
-  float s = (most >= -least ? most : least) * -0.125f;
-  if (s > 65504.f) s = 65504.f;
-  if (s < -65504.f) s = -65504.f;
-  const __half h = __float2half_rn(s);
-  return __half2float(h) == 0.f ? __ushort_as_half(0) : h;    // no negative zero
-}
-
 struct Q4Scale {
   __half half;
-  float inv;
+  float inv;                    // its reciprocal, within 2^-23
   bool plain;                   // the largest element is -8 scales exactly: no code can be below 0
 };
+// From the extremes of a group; a NaN among the elements makes both NaN.
 __device__ __forceinline__ Q4Scale q4_group(float most, float least) {
+  const float m = most >= -least ? most : least;
   Q4Scale s;
-  s.half = q4_scale(most, least);
-  const float scale = __half2float(s.half), m = most >= -least ? most : least;
-  s.inv = scale != 0.f ? __frcp_rn(scale) : 0.f;
-  s.plain = scale * -8.f == m;
+  s.half = __float2half_rn(fmaf(m, -0.125f, 0.f));            // the sum has no negative zero
+  const float scale = __half2float(s.half);
+  s.plain = scale * -8.f == m && fabsf(m) <= 524032.f;      // an infinity is not
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.inv) : "f"(scale));
+  if (scale == 0.f) s.inv = 0.f;
+  if (!s.plain) {                                             // rounded (tiny groups), too large for fp16, NaN
+    float x = m * -0.125f;
+    if (x > 65504.f) x = 65504.f;
+    if (x < -65504.f) x = -65504.f;
+    s.half = __float2half_rn(x);
+    if (__half2float(s.half) == 0.f) s.half = __ushort_as_half(0);
+  }
   return s;
 }
 
-// N codes (at most 8) of a group, lowest nibble first.
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+
+// N codes (at most 8) of a plain group, lowest nibble first.
 template <int N>
-__device__ __forceinline__ uint32_t q4_codes(const float (&x)[N], const Q4Scale& s) {
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[N], float inv) {
+  // float bits of 1.5 * 2^23 + code: the constant part of each is taken off the sum
+  constexpr uint32_t kOnes = N == 8 ? 0x11111111u : N == 4 ? 0x1111u : 0u;
   uint32_t word = 0;
-  if (s.plain) {
-    // float bits of 1.5 * 2^23 + code: the constant part of each is taken off the sum
-    constexpr uint32_t kOnes = N == 8 ? 0x11111111u : N == 4 ? 0x1111u : 0u;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      word += __float_as_uint(fminf(fmaf(x[i], s.inv, 48.f), 55.f) + (12582912.f - 40.f)) << (4 * i);
-    return word - 0x4b400000u * kOnes;
+  for (int i = 0; i < N; i += 2) {
+    float2 y = ffma2(make_float2(x[i], x[i + 1]), make_float2(inv, inv), make_float2(48.f, 48.f));
+    y = fadd2(make_float2(fminf(y.x, 55.f), fminf(y.y, 55.f)), make_float2(12582912.f - 40.f, 12582912.f - 40.f));
+    word += (__float_as_uint(y.x) << (4 * i)) + (__float_as_uint(y.y) << (4 * i + 4));
   }
-  // a scale that fp16 rounded (tiny or huge groups), no scale at all, NaN and infinities
-  const float scale = __half2float(s.half);
+  return word - 0x4b400000u * kOnes;
+}
+// Of any group: a scale that fp16 rounded (tiny or huge groups), no scale at all, NaN and infinities.
+__device__ __noinline__ uint32_t q4_codes_any(float scale, float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7) {
+  const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+  uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float y = scale == 0.f ? 0.f : __fdiv_rn(x[i], scale);
     word |= (uint32_t)(min(max(__float2int_rn(y), -8), 7) + 8) << (4 * i);   // NaN converts to 0: code 8
   }
@@ -112,17 +128,20 @@ __device__ __forceinline__ Q4Window q4_window(const long long* slots, long long 
   return w;
 }
 
-// 8 neighbouring elements of a token's keys (pieces 0 .. hd / 8 - 1) or values (the rest); the four threads of a group are
-// neighbours and all lanes of the warp take part.
+// A piece: 8 neighbouring elements of a token's keys (pieces 0 .. hd / 8 - 1) or values (the rest). The four threads of a group
+// are neighbours and all lanes of the warp take part.
+__device__ __forceinline__ const uint16_t* q4_piece_of(const uint16_t* k, const uint16_t* v, long long t, int h, int piece, int hd,
+                                                       long long k_stride, long long v_stride) {
+  const int per = hd / 8;
+  return (piece >= per ? v + t * v_stride + (piece - per) * 8 : k + t * k_stride + piece * 8) + h * hd;
+}
+// Out of line where a kernel has it beside other work: what runs once a launch costs the fetching of its instructions.
 template <bool BF16>
-__device__ __forceinline__ void q4_put_piece(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint8_t* __restrict__ pool,
-                                             long long t, long long slot, int h, int piece, bool live, int hkv, int hd, int tiles,
-                                             long long k_stride, long long v_stride) {
+__device__ __noinline__ void q4_put_piece(const uint4& u, uint8_t* __restrict__ pool, long long slot, int h, int piece, bool live,
+                                             int hkv, int hd, int tiles) {
   const int per = hd / 8, ng = hd / 32;
   const bool value = piece >= per;
   const int chunk = value ? piece - per : piece;
-  uint4 u = make_uint4(0u, 0u, 0u, 0u);
-  if (live) u = *reinterpret_cast<const uint4*>((value ? v + t * v_stride : k + t * k_stride) + h * hd + chunk * 8);
   float x[8];
   widen8<BF16>(u, x);
   float most = x[0], least = x[0];
@@ -138,7 +157,8 @@ __device__ __forceinline__ void q4_put_piece(const uint16_t* __restrict__ k, con
   }
   if (!live) return;
   const Q4Scale s = q4_group(most, least);
-  const uint32_t word = q4_codes(x, s);
+  const uint32_t word = s.plain ? q4_codes(x, s.inv)
+                                : q4_codes_any(__half2float(s.half), x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
   uint8_t* tile = pool + q4_tile_of(slot, h, hkv, tiles, q4_tile_bytes(hd));
   const int tok = (int)(slot & 15);
   if (value) {
@@ -161,116 +181,213 @@ kv_append_q4_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__
   const long long th = i / per, t = th / hkv;
   const int h = (int)(th % hkv);
   const long long slot = i < total ? slots[t] : -1;
-  q4_put_piece<BF16>(k, v, pool, t, slot, h, piece, slot >= 0 && slot < num_slots, hkv, hd, tiles, k_stride, v_stride);
+  const bool live = slot >= 0 && slot < num_slots;
+  uint4 u = make_uint4(0u, 0u, 0u, 0u);
+  if (live) u = *reinterpret_cast<const uint4*>(q4_piece_of(k, v, t, h, piece, hd, k_stride, v_stride));
+  q4_put_piece<BF16>(u, pool, slot, h, piece, live, hkv, hd, tiles);
 }
 
-__device__ __forceinline__ void q4_extremes2(uint32_t u, uint32_t& most, uint32_t& least, bool bf16) {
-  if (bf16) {
-    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(most) : "r"(u));
-    asm("min.NaN.bf16x2 %0, %0, %1;" : "+r"(least) : "r"(u));
-  } else {
-    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(most) : "r"(u));
-    asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(least) : "r"(u));
-  }
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 template <bool BF16>
 __device__ __forceinline__ float2 widen2(uint32_t u) {
   return BF16 ? unpack_bf16x2(u) : __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-// Scale of a group whose W registers are here, the rest in the lanes that differ in the bits OFF1 .. OFF2.
+// Scale of a group whose W registers are here, the rest in the lanes that differ in the bits OFF1 .. OFF2. The largest element
+// and the largest negated one travel in one register.
 template <bool BF16, int W, int OFF1, int OFF2>
 __device__ __forceinline__ Q4Scale q4_group_of(const uint32_t* u) {
   uint32_t most = u[0], least = u[0];
 #pragma unroll
-  for (int i = 1; i < W; ++i) q4_extremes2(u[i], most, least, BF16);
-#pragma unroll
-  for (int off = OFF1; off <= OFF2; off <<= 1) {
-    const uint32_t a = __shfl_xor_sync(0xffffffffu, most, off), b = __shfl_xor_sync(0xffffffffu, least, off);
-    uint32_t none = a;
-    q4_extremes2(a, most, none, BF16);
-    none = b;
-    q4_extremes2(b, none, least, BF16);
+  for (int i = 1; i < W; ++i) {
+    most = max2<BF16>(most, u[i]);
+    least = min2<BF16>(least, u[i]);
   }
-  const float2 a = widen2<BF16>(most), b = widen2<BF16>(least);
-  return q4_group(max_nan(a.x, a.y), min_nan(b.x, b.y));
+  // (most, -least) of the even and of the odd elements
+  least ^= 0x80008000u;
+  uint32_t both = max2<BF16>(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
+#pragma unroll
+  for (int off = OFF1; off <= OFF2; off <<= 1) both = max2<BF16>(both, __shfl_xor_sync(0xffffffffu, both, off));
+  const float2 m = widen2<BF16>(both);
+  return q4_group(m.x, -m.y);
+}
+// NG fp16 scales at once (p aligned to them).
+template <int NG>
+__device__ __forceinline__ void put_scales(__half* p, const __half (&s)[NG]) {
+  if (NG == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(s);
+  else if (NG == 4) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(s);
+  else {
+#pragma unroll
+    for (int i = 0; i < NG; i += 2) *reinterpret_cast<uint32_t*>(p + i) = *reinterpret_cast<const uint32_t*>(s + i);
+  }
+}
+template <int NG>
+__device__ __forceinline__ void get_scales(const __half* p, __half (&s)[NG]) {
+  if (NG == 8) *reinterpret_cast<uint4*>(s) = *reinterpret_cast<const uint4*>(p);
+  else if (NG == 4) *reinterpret_cast<uint2*>(s) = *reinterpret_cast<const uint2*>(p);
+  else {
+#pragma unroll
+    for (int i = 0; i < NG; i += 2) *reinterpret_cast<uint32_t*>(s + i) = *reinterpret_cast<const uint32_t*>(p + i);
+  }
+}
+
+// The words i0 .. i0 + NG - 1 of this lane in one half of a tile.
+template <int NG>
+__device__ __forceinline__ void put_words(uint8_t* half, int i0, const uint32_t (&w)[NG]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < NG; i += (NG % 4 == 0 ? 4 : 2)) {
+    uint8_t* to = half + q4_word_at(i0 + i, lane);
+    if (NG % 4 == 0) *reinterpret_cast<uint4*>(to) = make_uint4(w[i], w[i + 1], w[(i + 2) % NG], w[(i + 3) % NG]);
+    else *reinterpret_cast<uint2*>(to) = make_uint2(w[i], w[i + 1]);
+  }
+}
+template <int NG>
+__device__ __forceinline__ void get_words(const uint8_t* half, int i0, uint32_t (&w)[NG]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < NG; i += (NG % 4 == 0 ? 4 : 2)) {
+    const uint8_t* from = half + q4_word_at(i0 + i, lane);
+    if (NG % 4 == 0) {
+      const uint4 u = *reinterpret_cast<const uint4*>(from);
+      w[i] = u.x; w[i + 1] = u.y; w[(i + 2) % NG] = u.z; w[(i + 3) % NG] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(from);
+      w[i] = u.x; w[i + 1] = u.y;
+    }
+  }
 }
 
 constexpr int kQ4RowWarps = 4;
 
-// Grid (16-row windows, heads / 4): a warp has one head.
+// Grid (16-row windows, heads). A tile's work is shared by four warps: keys and values, first and second 8 tokens.
 template <int NG, bool BF16>
 __global__ void __launch_bounds__(kQ4RowWarps * 32)
 kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint8_t* __restrict__ pool,
                          const long long* __restrict__ slots, long long T, int hkv, int tiles, long long num_slots,
-                         long long k_stride, long long v_stride) {
-  constexpr int HD = NG * 32;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y * kQ4RowWarps + (threadIdx.x >> 5);
-  if (h >= hkv) return;
+                         long long k_stride, long long v_stride, int per) {
+  constexpr int HD = NG * 32, PIECES = (HD / 4 + 31) / 32, DEPTH = 4;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   const long long first = (long long)blockIdx.x * 16;
   const Q4Window w = q4_window(slots, first, T, num_slots);
-  if (w.leader >= 0) {
-    const long long t0 = first + w.leader;
-    uint8_t* tile = pool + q4_tile_of(__shfl_sync(0xffffffffu, w.slot, w.leader), h, hkv, tiles, 18 * HD);
-    __half* scales = reinterpret_cast<__half*>(tile + 16 * HD);
-    uint32_t word[2 * NG];
-    // keys: tokens r, r + 8, elements 32 g + 8 c ..
+#pragma unroll 1
+  for (int h = blockIdx.y * per; h < min(hkv, (int)(blockIdx.y + 1) * per); ++h) {
+    // rows that go one by one: bit i for row row0 + i, whose slot lane i has; pieces p0 to p1 of them
+    long long row0 = first, slot = w.slot;
+    uint32_t left = 0;
+    int p0 = 0, p1 = HD / 4;
+    if (w.leader >= 0) {
+      const long long t0 = first + w.leader, slot0 = __shfl_sync(0xffffffffu, w.slot, w.leader);
+      uint8_t* tile = pool + q4_tile_of(slot0, h, hkv, tiles, 18 * HD);
+      __half* scales = reinterpret_cast<__half*>(tile + 16 * HD);
+      const int j = warp & 1;
+      uint32_t word[NG];
+      bool plain = true;
+      if (warp < 2) {                              // keys: token 8 j + r, elements 32 g + 8 c ..
+        const int tok = 8 * j + r;
+        const uint16_t* from = k + (t0 + tok) * k_stride + h * HD + c * 8;
+        uint4 u[NG];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint16_t* from = k + (t0 + r + 8 * j) * k_stride + h * HD + c * 8;
-      uint4 u[NG];
+        for (int g = 0; g < NG; ++g) u[g] = *reinterpret_cast<const uint4*>(from + g * 32);
+        __align__(16) __half row[NG];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) u[g] = *reinterpret_cast<const uint4*>(from + g * 32);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t x2[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
-        const Q4Scale s = q4_group_of<BF16, 4, 1, 2>(x2);
-        float x[8];
-        widen8<BF16>(u[g], x);
-        word[j * NG + g] = q4_codes(x, s);
-        if (c == 0) scales[(r + 8 * j) * 2 * NG + g] = s.half;
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < NG / 2; ++p)
-      *reinterpret_cast<uint4*>(tile + p * 512 + lane * 16) = make_uint4(word[4 * p], word[4 * p + 1], word[4 * p + 2], word[4 * p + 3]);
-    // values: tokens 8 j + 2 c, + 1, elements 32 g + 4 r ..
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint2 u[2][NG];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint16_t* from = v + (t0 + 8 * j + 2 * c + e) * v_stride + h * HD + r * 4;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) u[e][g] = *reinterpret_cast<const uint2*>(from + g * 32);
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint32_t both = 0;
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t x2[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
+          const Q4Scale s = q4_group_of<BF16, 4, 1, 2>(x2);
+          float x[8];
+          widen8<BF16>(u[g], x);
+          word[g] = q4_codes(x, s.inv);
+          row[g] = s.half;
+          plain &= s.plain;
+        }
+        put_words<NG>(tile, j * NG, word);
+        if (c == 0) put_scales<NG>(scales + tok * 2 * NG, row);
+        p1 = HD / 8;
+      } else {                                     // values: tokens 8 j + 2 c, + 1, elements 32 g + 4 r ..
+        const int tok = 8 * j + 2 * c;
+        uint2 u[2][NG];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t x2[2] = {u[e][g].x, u[e][g].y};
-          const Q4Scale s = q4_group_of<BF16, 2, 4, 16>(x2);
-          const float2 lo = widen2<BF16>(x2[0]), hi = widen2<BF16>(x2[1]);
-          const float x[4] = {lo.x, lo.y, hi.x, hi.y};
-          both |= q4_codes(x, s) << (16 * e);
-          if (r == 0) scales[(8 * j + 2 * c + e) * 2 * NG + NG + g] = s.half;
+          const uint16_t* from = v + (t0 + tok + e) * v_stride + h * HD + r * 4;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) u[e][g] = *reinterpret_cast<const uint2*>(from + g * 32);
         }
-        word[j * NG + g] = both;
+        __align__(16) __half row[2][NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint32_t both = 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x2[2] = {u[e][g].x, u[e][g].y};
+            const Q4Scale s = q4_group_of<BF16, 2, 4, 16>(x2);
+            const float2 lo = widen2<BF16>(x2[0]), hi = widen2<BF16>(x2[1]);
+            const float x[4] = {lo.x, lo.y, hi.x, hi.y};
+            both |= q4_codes(x, s.inv) << (16 * e);
+            row[e][g] = s.half;
+            plain &= s.plain;
+          }
+          word[g] = both;
+        }
+        put_words<NG>(tile + 8 * HD, j * NG, word);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (r == 0) put_scales<NG>(scales + (tok + e) * 2 * NG + NG, row[e]);
+        p0 = HD / 8;
+      }
+      if (!__all_sync(0xffffffffu, plain)) {       // a group needs the long way: the warp's part takes it, over what it wrote
+        __syncwarp();
+        row0 = t0;
+        slot = slot0 + (lane & 15);
+        left = 0xffu << (8 * j);
       }
     }
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {         // the warp's part once more, then its share of the rows that fill no tile
+      while (left != 0u) {
+        uint4 u[DEPTH][PIECES];                    // some rows at a time, so that their loads share a wait
+        uint32_t rest = left;
 #pragma unroll
-    for (int p = 0; p < NG / 2; ++p)
-      *reinterpret_cast<uint4*>(tile + 8 * HD + p * 512 + lane * 16) =
-          make_uint4(word[4 * p], word[4 * p + 1], word[4 * p + 2], word[4 * p + 3]);
-  }
-  for (int i = 0; i < 16; ++i) {
-    if (w.covered >> i & 1) continue;
-    const long long slot = __shfl_sync(0xffffffffu, w.slot, i);
-    if (slot < 0 || slot >= num_slots) continue;
+        for (int i = 0; i < DEPTH; ++i) {
+          const int row = __ffs(rest) - 1;
 #pragma unroll
-    for (int p = 0; p < HD / 4; p += 32)
-      q4_put_piece<BF16>(k, v, pool, first + i, slot, h, p + lane, p + lane < HD / 4, hkv, HD, tiles, k_stride, v_stride);
+          for (int p = 0; p < PIECES; ++p) {
+            const int piece = p0 + p * 32 + lane;
+            u[i][p] = make_uint4(0u, 0u, 0u, 0u);
+            if (row >= 0 && piece < p1) u[i][p] = *reinterpret_cast<const uint4*>(q4_piece_of(k, v, row0 + row, h, piece, HD, k_stride, v_stride));
+          }
+          rest &= rest - 1;
+        }
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+          if (left == 0u) break;
+          const long long at = __shfl_sync(0xffffffffu, slot, __ffs(left) - 1);
+#pragma unroll
+          for (int p = 0; p < PIECES; ++p) {
+            const int piece = p0 + p * 32 + lane;
+            q4_put_piece<BF16>(u[i][p], pool, at, h, piece, piece < p1, hkv, HD, tiles);
+          }
+          left &= left - 1;
+        }
+      }
+      if (turn == 1) break;
+      row0 = first;
+      slot = w.slot;
+      p0 = 0;
+      p1 = HD / 4;
+      left = __ballot_sync(0xffffffffu, lane < 16 && slot >= 0 && slot < num_slots) & ~w.covered & (0x1111u << warp);
+    }
   }
 }
 
@@ -286,29 +403,35 @@ __device__ __forceinline__ uint2 q4_values4(uint32_t codes, float scale) {
   return make_uint2(q4_value2<BF16>(codes & 15u, codes >> 4 & 15u, scale), q4_value2<BF16>(codes >> 8 & 15u, codes >> 12 & 15u, scale));
 }
 
-template <bool BF16>
-__device__ __forceinline__ void q4_get_piece(const uint8_t* __restrict__ pool, uint16_t* __restrict__ k, uint16_t* __restrict__ v,
-                                             long long t, long long slot, int h, int piece, bool live, int hkv, int hd, int tiles) {
+struct Q4Piece {
+  uint32_t word;
+  __half scale;
+};
+__device__ __forceinline__ Q4Piece q4_get_piece(const uint8_t* __restrict__ pool, long long slot, int h, int piece, bool live, int hkv,
+                                                int hd, int tiles) {
+  Q4Piece x{0x88888888u, __ushort_as_half(0)};    // zeros
+  if (!live) return x;
   const int per = hd / 8, ng = hd / 32;
   const bool value = piece >= per;
-  const int chunk = value ? piece - per : piece;
-  uint4 out = make_uint4(0u, 0u, 0u, 0u);
-  if (live) {
-    const uint8_t* tile = pool + q4_tile_of(slot, h, hkv, tiles, q4_tile_bytes(hd));
-    const int tok = (int)(slot & 15);
-    uint32_t word;
-    if (value) {
-      const uint8_t* half = tile + 8 * hd;
-      word = *reinterpret_cast<const uint16_t*>(half + q4_value_at(ng, tok, 2 * chunk)) |
+  const int chunk = value ? piece - per : piece, tok = (int)(slot & 15);
+  const uint8_t* tile = pool + q4_tile_of(slot, h, hkv, tiles, q4_tile_bytes(hd));
+  if (value) {
+    const uint8_t* half = tile + 8 * hd;
+    x.word = *reinterpret_cast<const uint16_t*>(half + q4_value_at(ng, tok, 2 * chunk)) |
              (uint32_t)*reinterpret_cast<const uint16_t*>(half + q4_value_at(ng, tok, 2 * chunk + 1)) << 16;
-    } else {
-      word = *reinterpret_cast<const uint32_t*>(tile + q4_key_at(ng, tok, chunk));
-    }
-    const float scale = __half2float(reinterpret_cast<const __half*>(tile + 16 * hd)[tok * 2 * ng + (value ? ng : 0) + (chunk >> 2)]);
-    const uint2 a = q4_values4<BF16>(word & 0xffffu, scale), b = q4_values4<BF16>(word >> 16, scale);
-    out = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    x.word = *reinterpret_cast<const uint32_t*>(tile + q4_key_at(ng, tok, chunk));
   }
-  *reinterpret_cast<uint4*>((value ? v : k) + (t * hkv + h) * hd + chunk * 8) = out;
+  x.scale = reinterpret_cast<const __half*>(tile + 16 * hd)[tok * 2 * ng + (value ? ng : 0) + (chunk >> 2)];
+  return x;
+}
+template <bool BF16>
+__device__ __forceinline__ void q4_write_piece(const Q4Piece& x, uint16_t* __restrict__ k, uint16_t* __restrict__ v, long long t,
+                                               int h, int piece, int hkv, int hd) {
+  const int per = hd / 8;
+  const float scale = __half2float(x.scale);
+  const uint2 a = q4_values4<BF16>(x.word & 0xffffu, scale), b = q4_values4<BF16>(x.word >> 16, scale);
+  *reinterpret_cast<uint4*>((piece >= per ? v + (piece - per) * 8 : k + piece * 8) + (t * hkv + h) * hd) = make_uint4(a.x, a.y, b.x, b.y);
 }
 
 template <bool BF16>
@@ -320,63 +443,89 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, const long long* __restrict_
   const int per = hd / 4, piece = (int)(i % per);
   const long long th = i / per, t = th / hkv;
   const long long slot = slots[t];
-  q4_get_piece<BF16>(pool, k, v, t, slot, (int)(th % hkv), piece, slot >= 0 && slot < num_slots, hkv, hd, tiles);
+  const int h = (int)(th % hkv);
+  q4_write_piece<BF16>(q4_get_piece(pool, slot, h, piece, slot >= 0 && slot < num_slots, hkv, hd, tiles), k, v, t, h, piece, hkv, hd);
 }
 
 template <int NG, bool BF16>
 __global__ void __launch_bounds__(kQ4RowWarps * 32)
 kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __restrict__ slots, uint16_t* __restrict__ k,
-                       uint16_t* __restrict__ v, long long T, int hkv, int tiles, long long num_slots) {
-  constexpr int HD = NG * 32;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y * kQ4RowWarps + (threadIdx.x >> 5);
-  if (h >= hkv) return;
+                       uint16_t* __restrict__ v, long long T, int hkv, int tiles, long long num_slots, int per) {
+  constexpr int HD = NG * 32, PIECES = (HD / 4 + 31) / 32, DEPTH = 4;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   const long long first = (long long)blockIdx.x * 16;
   const Q4Window w = q4_window(slots, first, T, num_slots);
-  if (w.leader >= 0) {
-    const long long t0 = first + w.leader, pitch = (long long)hkv * HD;
-    const uint8_t* tile = pool + q4_tile_of(__shfl_sync(0xffffffffu, w.slot, w.leader), h, hkv, tiles, 18 * HD);
-    const __half* scales = reinterpret_cast<const __half*>(tile + 16 * HD);
-    uint32_t kw[2 * NG], vw[2 * NG];
+#pragma unroll 1
+  for (int h = blockIdx.y * per; h < min(hkv, (int)(blockIdx.y + 1) * per); ++h) {
+    if (w.leader >= 0) {
+      const long long t0 = first + w.leader, pitch = (long long)hkv * HD;
+      const uint8_t* tile = pool + q4_tile_of(__shfl_sync(0xffffffffu, w.slot, w.leader), h, hkv, tiles, 18 * HD);
+      const __half* scales = reinterpret_cast<const __half*>(tile + 16 * HD);
+      const int j = warp & 1;
+      uint32_t word[NG];
+      if (warp < 2) {                              // keys: token 8 j + r, elements 32 g + 8 c ..
+        const int tok = 8 * j + r;
+        __align__(16) __half row[NG];
+        get_words<NG>(tile, j * NG, word);
+        get_scales<NG>(scales + tok * 2 * NG, row);
+        uint16_t* to = k + (t0 + tok) * pitch + h * HD + c * 8;
 #pragma unroll
-    for (int p = 0; p < NG / 2; ++p) {
-      const uint4 a = *reinterpret_cast<const uint4*>(tile + p * 512 + lane * 16);
-      const uint4 b = *reinterpret_cast<const uint4*>(tile + 8 * HD + p * 512 + lane * 16);
-      kw[4 * p] = a.x; kw[4 * p + 1] = a.y; kw[4 * p + 2] = a.z; kw[4 * p + 3] = a.w;
-      vw[4 * p] = b.x; vw[4 * p + 1] = b.y; vw[4 * p + 2] = b.z; vw[4 * p + 3] = b.w;
+        for (int g = 0; g < NG; ++g) {
+          const float scale = __half2float(row[g]);
+          const uint2 a = q4_values4<BF16>(word[g] & 0xffffu, scale), b = q4_values4<BF16>(word[g] >> 16, scale);
+          *reinterpret_cast<uint4*>(to + g * 32) = make_uint4(a.x, a.y, b.x, b.y);
+        }
+      } else {                                     // values: tokens 8 j + 2 c, + 1, elements 32 g + 4 r ..
+        const int tok = 8 * j + 2 * c;
+        __align__(16) __half row[2][NG];
+        get_words<NG>(tile + 8 * HD, j * NG, word);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) get_scales<NG>(scales + (tok + e) * 2 * NG + NG, row[e]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint16_t* to = v + (t0 + tok + e) * pitch + h * HD + r * 4;
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            *reinterpret_cast<uint2*>(to + g * 32) = q4_values4<BF16>(e ? word[g] >> 16 : word[g] & 0xffffu, __half2float(row[e][g]));
+        }
+      }
     }
+    // this warp's share of the rows that fill no tile, some at a time so that their loads share a wait
+    uint32_t left = ~w.covered & (first + 16 <= T ? 0xffffu : (1u << (T - first)) - 1u) & (0x1111u << warp);
+    while (left != 0u) {
+      Q4Piece x[DEPTH][PIECES];
+      uint32_t rest = left;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint16_t* to = k + (t0 + r + 8 * j) * pitch + h * HD + c * 8;
+      for (int i = 0; i < DEPTH; ++i) {
+        const int row = __ffs(rest) - 1;
+        const long long slot = __shfl_sync(0xffffffffu, w.slot, max(row, 0));
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float scale = __half2float(scales[(r + 8 * j) * 2 * NG + g]);
-        const uint32_t word = kw[j * NG + g];
-        const uint2 a = q4_values4<BF16>(word & 0xffffu, scale), b = q4_values4<BF16>(word >> 16, scale);
-        *reinterpret_cast<uint4*>(to + g * 32) = make_uint4(a.x, a.y, b.x, b.y);
+        for (int p = 0; p < PIECES; ++p)
+          x[i][p] = q4_get_piece(pool, slot, h, p * 32 + lane, row >= 0 && p * 32 + lane < HD / 4 && slot >= 0 && slot < num_slots, hkv, HD, tiles);
+        rest &= rest - 1;
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int tok = 8 * j + 2 * c + e;
-        uint16_t* out = v + (t0 + tok) * pitch + h * HD + r * 4;
+      for (int i = 0; i < DEPTH; ++i) {
+        if (left == 0u) break;
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-          *reinterpret_cast<uint2*>(out + g * 32) =
-              q4_values4<BF16>(e ? vw[j * NG + g] >> 16 : vw[j * NG + g] & 0xffffu, __half2float(scales[tok * 2 * NG + NG + g]));
+        for (int p = 0; p < PIECES; ++p)
+          if (p * 32 + lane < HD / 4) q4_write_piece<BF16>(x[i][p], k, v, first + __ffs(left) - 1, h, p * 32 + lane, hkv, HD);
+        left &= left - 1;
       }
     }
-  }
-  for (int i = 0; i < 16 && first + i < T; ++i) {
-    if (w.covered >> i & 1) continue;
-    const long long slot = __shfl_sync(0xffffffffu, w.slot, i);
-    for (int p = lane; p < HD / 4; p += 32)
-      q4_get_piece<BF16>(pool, k, v, first + i, slot, h, p, slot >= 0 && slot < num_slots, hkv, HD, tiles);
   }
 }
 
 // Rows from which on the kernels by tiles take a call. Few rows are a decode step's, no two of them in a tile, or a prompt that
 // one launch of either kind is too short for.
 constexpr long long kQ4TileRows = 512;
+
+// Heads that a block goes through one after the other, so that its look at the slots serves them all; blocks stay enough for
+// sixteen to an SM.
+static int q4_heads_per_block(long long T, int hkv) {
+  const long long all = (T + 15) / 16 * hkv, per = all / (16LL * num_sms());
+  return per < 1 ? 1 : per < hkv ? (int)per : hkv;
+}
 
 }  // namespace icb
 
@@ -403,11 +552,12 @@ ICB_API int icb_kv_append_q4(const void* k, const void* v, void* pool, const lon
   auto p = reinterpret_cast<uint8_t*>(pool);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (T >= kQ4TileRows) {
-    const dim3 grid((unsigned)((T + 15) / 16), (hkv + kQ4RowWarps - 1) / kQ4RowWarps);
+    const int per = q4_heads_per_block(T, hkv);
+    const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
     if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) \
-    if (dtype == kBF16) kv_append_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride); \
-    else kv_append_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride);
+    if (dtype == kBF16) kv_append_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride, per); \
+    else kv_append_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride, per);
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
   } else {
@@ -429,11 +579,12 @@ ICB_API int icb_kv_read_q4(const void* pool, const long long* slots, void* k, vo
   auto p = reinterpret_cast<const uint8_t*>(pool);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (T >= kQ4TileRows) {
-    const dim3 grid((unsigned)((T + 15) / 16), (hkv + kQ4RowWarps - 1) / kQ4RowWarps);
+    const int per = q4_heads_per_block(T, hkv);
+    const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
     if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) \
-    if (dtype == kBF16) kv_read_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots); \
-    else kv_read_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots);
+    if (dtype == kBF16) kv_read_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots, per); \
+    else kv_read_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots, per);
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
   } else {
