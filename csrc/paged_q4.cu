@@ -64,14 +64,15 @@ __device__ __forceinline__ Q4Scale q4_group(float most, float least) {
   return s;
 }
 
+__device__ __forceinline__ unsigned long long bits2(const float2& a) { return *reinterpret_cast<const unsigned long long*>(&a); }
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
   return *reinterpret_cast<float2*>(&d);
 }
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
   return *reinterpret_cast<float2*>(&d);
 }
 
@@ -272,7 +273,7 @@ __device__ __forceinline__ void get_words(const uint8_t* half, int i0, uint32_t 
 
 constexpr int kQ4RowWarps = 4;
 
-// Grid (16-row windows, heads). A tile's work is shared by four warps: keys and values, first and second 8 tokens.
+// Grid (16-row windows, runs of heads). A tile's work is shared by four warps: keys and values, first and second 8 tokens.
 template <int NG, bool BF16>
 __global__ void __launch_bounds__(kQ4RowWarps * 32)
 kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint8_t* __restrict__ pool,
@@ -516,9 +517,10 @@ kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __rest
   }
 }
 
-// Rows from which on the kernels by tiles take a call. Few rows are a decode step's, no two of them in a tile, or a prompt that
-// one launch of either kind is too short for.
-constexpr long long kQ4TileRows = 512;
+// Elements of the keys from which on the kernels by tiles take a call. Below, a call is a decode step, whose rows lie in a tile
+// each, or too short for either kind to fill the GPU. In order, append by rows / by tiles: 8 heads of 128, 512 rows 7.4 / 9.4
+// us, 2048 rows 12.3 / 10.2, 8192 rows 31 / 21, 32768 rows 104 / 51; 1 head of 256, 8192 rows 12.3 / 14.4, 32768 rows 29 / 19.
+constexpr long long kQ4TileElements = 1LL << 21;
 
 // Heads that a block goes through one after the other, so that its look at the slots serves them all; blocks stay enough for
 // sixteen to an SM.
@@ -551,7 +553,7 @@ ICB_API int icb_kv_append_q4(const void* k, const void* v, void* pool, const lon
   auto K = reinterpret_cast<const uint16_t*>(k), V = reinterpret_cast<const uint16_t*>(v);
   auto p = reinterpret_cast<uint8_t*>(pool);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (T >= kQ4TileRows) {
+  if (T * hkv * hd >= kQ4TileElements) {
     const int per = q4_heads_per_block(T, hkv);
     const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
     if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
@@ -578,7 +580,7 @@ ICB_API int icb_kv_read_q4(const void* pool, const long long* slots, void* k, vo
   auto K = reinterpret_cast<uint16_t*>(k), V = reinterpret_cast<uint16_t*>(v);
   auto p = reinterpret_cast<const uint8_t*>(pool);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (T >= kQ4TileRows) {
+  if (T * hkv * hd >= kQ4TileElements) {
     const int per = q4_heads_per_block(T, hkv);
     const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
     if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;

@@ -25,7 +25,8 @@ def _rows(t, hkv, hd, dtype, seed=0, device="cuda"):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("hkv,hd,bs,t", [(2, 128, 16, 1), (12, 64, 32, 77), (1, 256, 16, 300), (3, 192, 48, 130), (8, 128, 64, 1000)])
+@pytest.mark.parametrize("hkv,hd,bs,t", [(2, 128, 16, 1), (12, 64, 32, 77), (1, 256, 16, 300), (3, 192, 48, 130), (8, 128, 64, 1000),
+                                         (8, 128, 64, 2100), (2, 256, 16, 4200), (12, 64, 32, 2800), (5, 192, 48, 2200)])
 def test_append_and_read(hkv, hd, bs, t, dtype):
     from ironcore_b200.ops import paged
 
@@ -73,6 +74,32 @@ def test_append_extreme_groups():
             assert torch.equal(x.cpu().nan_to_num(7.0), y.nan_to_num(7.0))
         codes = 16 * 64                                     # NaN scales may differ in their bits, codes may not
         assert torch.equal(got.cpu()[..., :codes], want[..., :codes])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_extreme_groups_among_many_rows(dtype):
+    """Whole tiles with a group that fp16 scales do not hold exactly, that has none, or that is not finite."""
+    from ironcore_b200.ops import paged
+
+    hkv, hd, t = 8, 128, 2304
+    k, v = (x.clone() for x in _rows(t, hkv, hd, dtype, seed=9, device="cpu"))
+    for i, (x, value) in enumerate([(k, float("nan")), (v, float("-inf")), (v, float("nan")), (k, 3e38), (v, float("inf")), (k, 0.0)]):
+        x[100 + 37 * i, 64 + i] = value
+    for i, x in enumerate((k, v, k, v)):
+        x[900 + 50 * i, 128:160] = torch.linspace(-3, 2.9, 32).to(dtype) * 2.0 ** -(23 + i)
+        x[1500 + 50 * i, 32 * i:32 * i + 64] = 0
+    blocks = t // 16 + 2
+    slots = torch.randperm(blocks, generator=torch.Generator().manual_seed(0))[torch.arange(t) // 16] * 16 + torch.arange(t) % 16
+    want = torch.zeros(paged.q4_pool_shape(blocks, hkv, 16, hd), dtype=torch.uint8)
+    got = want.cuda()
+    paged.kv_append_q4_reference(k, v, want, slots)
+    paged.kv_append_q4(k.cuda(), v.cuda(), got, slots.cuda())
+    codes = 16 * hd
+    assert torch.equal(got.cpu()[..., :codes], want[..., :codes])
+    scales = [x.cpu()[..., codes:].contiguous().view(HF) for x in (got, want)]
+    assert torch.equal(scales[0].isnan(), scales[1].isnan()) and torch.equal(scales[0].nan_to_num(), scales[1].nan_to_num())
+    for x, y in zip(paged.kv_read_q4(got, slots.cuda(), dtype), paged.kv_read_q4_reference(want, slots, dtype)):
+        assert torch.equal(x.cpu().nan_to_num(), y.nan_to_num()) and torch.equal(x.cpu().isnan(), y.isnan())
 
 
 def _check(q, pool, table, lens, hq, scale=None, **kw):
