@@ -8,8 +8,8 @@
 namespace icb {
 
 constexpr int kPageCopyPools = 96;        // pools of one launch (kernel parameters hold 4 KB)
-constexpr int kPageCopyThreads = 256;
-constexpr int kPageCopyDepth = 4;         // accesses in flight per thread
+constexpr int kPageCopyThreads = 128;
+constexpr int kPageCopyDepth = 5;         // accesses in flight per thread
 
 struct PagePool {
   uint8_t* base;
@@ -25,31 +25,35 @@ struct PageCopyArgs {
   int pools, pairs;
 };
 
-// A work item is one stretch of VEC-byte accesses of one page: item = ((pool, layer) * pairs + pair) * stretches + stretch.
+// A page is cut into the fewest equal stretches that a block moves with all its loads in flight. Equal: 4-bit pages of 18 KB and
+// the like would leave a short last stretch (448 pairs of 18 KB in 32 layers, from 64 pages: 58 us, now 51.5, 0.89 of the copy
+// bandwidth). Blocks that take neighbouring VECs across pages' borders need two divisions per access and wait for them (76 us).
+// 128 threads of 5 accesses: 8 KB pages, 448 pairs in 56 pools, 40.8 us; 256 of 4 45.5, 128 of 16 53.6.
+__host__ __device__ inline long long page_stretches(long long n) {
+  return (n + kPageCopyThreads * kPageCopyDepth - 1) / (kPageCopyThreads * kPageCopyDepth);
+}
+
 template <typename VEC>
 __global__ void __launch_bounds__(kPageCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyArgs a) {
-  constexpr int STRETCH = kPageCopyThreads * kPageCopyDepth;
-  const long long item = blockIdx.x;
+  const uint32_t item = blockIdx.x;
   int p = 0;
   while (p + 1 < a.pools && item >= a.pool[p + 1].first_item) ++p;
   const PagePool& pool = a.pool[p];
-  const long long n = pool.page_bytes / (long long)sizeof(VEC);
-  const long long stretches = (n + STRETCH - 1) / STRETCH;
-  const long long local = item - pool.first_item;
-  const long long unit = local / stretches;
-  const int layer = (int)(unit / a.pairs), pair = (int)(unit - (long long)layer * a.pairs);
+  const uint32_t n = (uint32_t)(pool.page_bytes / (long long)sizeof(VEC)), stretches = (uint32_t)page_stretches(n);
+  const uint32_t local = item - (uint32_t)pool.first_item, unit = local / stretches, each = (n + stretches - 1) / stretches;
+  const uint32_t layer = unit / a.pairs, pair = unit - layer * a.pairs;
   const int s = a.src[pair], d = a.dst[pair];
   if (s < 0 || d < 0 || s >= pool.num_pages || d >= pool.num_pages) return;
   const VEC* from = reinterpret_cast<const VEC*>(pool.base + layer * pool.layer_bytes + s * pool.page_bytes);
   VEC* to = reinterpret_cast<VEC*>(pool.base + layer * pool.layer_bytes + d * pool.page_bytes);
-  const long long at = (local - unit * stretches) * STRETCH + threadIdx.x;
+  const uint32_t at = (local - unit * stretches) * each + threadIdx.x, end = min(n, at - threadIdx.x + each);
   VEC x[kPageCopyDepth];
 #pragma unroll
   for (int i = 0; i < kPageCopyDepth; ++i)
-    if (at + i * kPageCopyThreads < n) x[i] = from[at + i * kPageCopyThreads];
+    if (at + i * kPageCopyThreads < end) x[i] = from[at + i * kPageCopyThreads];
 #pragma unroll
   for (int i = 0; i < kPageCopyDepth; ++i)
-    if (at + i * kPageCopyThreads < n) to[at + i * kPageCopyThreads] = x[i];
+    if (at + i * kPageCopyThreads < end) to[at + i * kPageCopyThreads] = x[i];
 }
 
 template <typename VEC>
@@ -57,8 +61,9 @@ static int launch_page_copy(PageCopyArgs& a, cudaStream_t st) {
   long long items = 0;
   for (int p = 0; p < a.pools; ++p) {
     const long long n = a.pool[p].page_bytes / (long long)sizeof(VEC);
+    if (n > 0x7fffffffLL) return -2;
     a.pool[p].first_item = items;
-    items += (n + kPageCopyThreads * kPageCopyDepth - 1) / (kPageCopyThreads * kPageCopyDepth) * a.pool[p].layers * a.pairs;
+    items += page_stretches(n) * a.pool[p].layers * a.pairs;
   }
   if (items <= 0) return 0;
   if (items > 0x7fffffffLL) return -3;

@@ -12,6 +12,8 @@
 // Both directions are bound by memory. Two forms each: one thread per 8 elements of a row, for few rows; and one warp per tile
 // of 16 rows and head in the order of the tile's lanes, so that all 18 hd bytes of the tile leave or arrive in 512-byte pieces
 // (a row by itself touches all of a tile's value sectors, two bytes in each). Rows that do not fill a tile go one by one.
+#include <string.h>
+
 #include "host_common.h"
 #include "ptx.cuh"
 #include "q4.cuh"
@@ -542,58 +544,72 @@ using namespace icb;
     default: return -3; \
   }
 
-// k, v: [T, hkv * hd] 16-bit rows of pitch k_stride / v_stride (16-byte aligned); pool: num_slots / (16 * tiles) pages of
-// [hkv][tiles] tiles; a row whose slot is negative or outside the pool is left out. hd 64, 128, 192 or 256.
-ICB_API int icb_kv_append_q4(const void* k, const void* v, void* pool, const long long* slots, long long T, int hkv, int hd,
-                             int tiles, long long num_slots, long long k_stride, long long v_stride, int dtype,
-                             void* stream) {
-  if (T <= 0) return 0;
-  if (hkv < 1 || hd % 64 || hd < 64 || hd > 256 || tiles < 1 || k_stride % 8 || v_stride % 8) return -2;
-  if (dtype != kBF16 && dtype != kF16) return -4;
-  auto K = reinterpret_cast<const uint16_t*>(k), V = reinterpret_cast<const uint16_t*>(v);
-  auto p = reinterpret_cast<uint8_t*>(pool);
+// The arguments of both entry points come as one record (a caller through ctypes spends a third of the time on it).
+//   k, v: [rows, hkv * hd] 16-bit rows of pitch k_stride / v_stride (16-byte aligned; read: contiguous); pool: num_slots /
+//   (16 * tiles) pages of [hkv][tiles] tiles; slots: int64 [rows]. hd 64, 128, 192 or 256.
+struct Q4RowsCall {
+  uint16_t *k, *v;
+  uint8_t* pool;
+  const long long* slots;
+  long long rows, hkv, hd, tiles, num_slots, k_stride, v_stride, dtype;
+};
+static int q4_rows_call(Q4RowsCall& c, const void* record) {
+  memcpy(&c, record, sizeof(c));
+  if (c.hkv < 1 || c.hkv > 0x7fffffffLL || c.tiles < 1 || c.tiles > 0x7fffffffLL || c.k_stride % 8 || c.v_stride % 8) return -2;
+  if (c.hd % 64 || c.hd < 64 || c.hd > 256) return -3;
+  return c.dtype == kBF16 || c.dtype == kF16 ? 0 : -4;
+}
+
+// Quantises rows into the pool; a row whose slot is negative or outside the pool is left out.
+ICB_API int icb_kv_append_q4(const void* record, void* stream) {
+  Q4RowsCall c;
+  const int bad = q4_rows_call(c, record);
+  if (bad) return bad;
+  if (c.rows <= 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (T * hkv * hd >= kQ4TileElements) {
-    const int per = q4_heads_per_block(T, hkv);
-    const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
-    if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
+  const int hkv = (int)c.hkv, hd = (int)c.hd, tiles = (int)c.tiles;
+  if (c.rows * hkv * hd >= kQ4TileElements) {
+    const int per = q4_heads_per_block(c.rows, hkv);
+    const dim3 grid((unsigned)((c.rows + 15) / 16), (hkv + per - 1) / per);
+    if ((c.rows + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) \
-    if (dtype == kBF16) kv_append_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride, per); \
-    else kv_append_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(K, V, p, slots, T, hkv, tiles, num_slots, k_stride, v_stride, per);
+    if (c.dtype == kBF16) \
+      kv_append_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(c.k, c.v, c.pool, c.slots, c.rows, hkv, tiles, c.num_slots, c.k_stride, c.v_stride, per); \
+    else \
+      kv_append_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(c.k, c.v, c.pool, c.slots, c.rows, hkv, tiles, c.num_slots, c.k_stride, c.v_stride, per);
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
   } else {
-    const long long total = T * hkv * (hd / 4), blocks = (total + 255) / 256;
+    const long long total = c.rows * hkv * (hd / 4), blocks = (total + 255) / 256;
     if (blocks > 0x7fffffffLL) return -3;
-    if (dtype == kBF16) kv_append_q4_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(K, V, p, slots, total, hkv, hd, tiles, num_slots, k_stride, v_stride);
-    else kv_append_q4_kernel<false><<<(unsigned)blocks, 256, 0, st>>>(K, V, p, slots, total, hkv, hd, tiles, num_slots, k_stride, v_stride);
+    auto kernel = c.dtype == kBF16 ? kv_append_q4_kernel<true> : kv_append_q4_kernel<false>;
+    kernel<<<(unsigned)blocks, 256, 0, st>>>(c.k, c.v, c.pool, c.slots, total, hkv, hd, tiles, c.num_slots, c.k_stride, c.v_stride);
   }
   return check_launch("kv_append_q4");
 }
 
-// The rows `slots` of the pool as 16-bit k, v [T, hkv * hd]; zeros for a slot outside the pool.
-ICB_API int icb_kv_read_q4(const void* pool, const long long* slots, void* k, void* v, long long T, int hkv, int hd,
-                           int tiles, long long num_slots, int dtype, void* stream) {
-  if (T <= 0) return 0;
-  if (hkv < 1 || hd % 64 || hd < 64 || hd > 256 || tiles < 1) return -2;
-  if (dtype != kBF16 && dtype != kF16) return -4;
-  auto K = reinterpret_cast<uint16_t*>(k), V = reinterpret_cast<uint16_t*>(v);
-  auto p = reinterpret_cast<const uint8_t*>(pool);
+// Rows of the pool in 16 bits; zeros for a slot outside the pool.
+ICB_API int icb_kv_read_q4(const void* record, void* stream) {
+  Q4RowsCall c;
+  const int bad = q4_rows_call(c, record);
+  if (bad) return bad;
+  if (c.rows <= 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (T * hkv * hd >= kQ4TileElements) {
-    const int per = q4_heads_per_block(T, hkv);
-    const dim3 grid((unsigned)((T + 15) / 16), (hkv + per - 1) / per);
-    if ((T + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
+  const int hkv = (int)c.hkv, hd = (int)c.hd, tiles = (int)c.tiles;
+  if (c.rows * hkv * hd >= kQ4TileElements) {
+    const int per = q4_heads_per_block(c.rows, hkv);
+    const dim3 grid((unsigned)((c.rows + 15) / 16), (hkv + per - 1) / per);
+    if ((c.rows + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) \
-    if (dtype == kBF16) kv_read_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots, per); \
-    else kv_read_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(p, slots, K, V, T, hkv, tiles, num_slots, per);
+    if (c.dtype == kBF16) kv_read_q4_tile_kernel<NG_, true><<<grid, kQ4RowWarps * 32, 0, st>>>(c.pool, c.slots, c.k, c.v, c.rows, hkv, tiles, c.num_slots, per); \
+    else kv_read_q4_tile_kernel<NG_, false><<<grid, kQ4RowWarps * 32, 0, st>>>(c.pool, c.slots, c.k, c.v, c.rows, hkv, tiles, c.num_slots, per);
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
   } else {
-    const long long total = T * hkv * (hd / 4), blocks = (total + 255) / 256;
+    const long long total = c.rows * hkv * (hd / 4), blocks = (total + 255) / 256;
     if (blocks > 0x7fffffffLL) return -3;
-    if (dtype == kBF16) kv_read_q4_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(p, slots, K, V, total, hkv, hd, tiles, num_slots);
-    else kv_read_q4_kernel<false><<<(unsigned)blocks, 256, 0, st>>>(p, slots, K, V, total, hkv, hd, tiles, num_slots);
+    auto kernel = c.dtype == kBF16 ? kv_read_q4_kernel<true> : kv_read_q4_kernel<false>;
+    kernel<<<(unsigned)blocks, 256, 0, st>>>(c.pool, c.slots, c.k, c.v, total, hkv, hd, tiles, c.num_slots);
   }
   return check_launch("kv_read_q4");
 }

@@ -18,6 +18,8 @@
 //     magnitude. Relative error 2^-11 down to 2^-26 of the largest contribution; sums, maxima and p itself stay in fp32.
 // Tokens outside the sequence get probability and value scale zero by selection, so nothing stale in a page (NaN scales
 // included) reaches a result. A page number outside the pool counts as a page outside the sequence.
+#include <string.h>
+
 #include "host_common.h"
 #include "ptx.cuh"
 #include "q4.cuh"
@@ -80,6 +82,19 @@ __device__ __forceinline__ void copy16(uint32_t smem, const void* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(global) : "memory");
 }
 
+// A tile (NG * 576 bytes) to shared memory, this lane's 16 of every 512 bytes; nothing if `there` is false.
+template <int NG>
+__device__ __forceinline__ void copy_tile(uint32_t smem, const uint8_t* global, bool there) {
+  constexpr int FULL = NG * 576 / 512;
+#pragma unroll
+  for (int i = 0; i < FULL; ++i)
+    asm volatile("{ .reg .pred p; setp.ne.s32 p, %2, 0; @p cp.async.cg.shared.global [%0], [%1], 16; }" ::"r"(smem + i * 512),
+                 "l"(global + i * 512), "r"((int)there) : "memory");
+  if (NG * 576 % 512 != 0)
+    asm volatile("{ .reg .pred p; setp.ne.s32 p, %2, 0; @p cp.async.cg.shared.global [%0], [%1], 16; }" ::"r"(smem + FULL * 512),
+                 "l"(global + FULL * 512), "r"((int)(there && (threadIdx.x & 31) * 16 < NG * 576 % 512)) : "memory");
+}
+
 template <bool BF16>
 __device__ __forceinline__ void q4_store4(uint16_t* to, float x, float y, float z, float w) {
   // rows of any pitch and alignment
@@ -98,15 +113,20 @@ __device__ __forceinline__ void q4_store4(uint16_t* to, float x, float y, float 
 
 // The query operand, resident in registers: column n of the matrix instructions is head n (T = 1, up to eight heads) or head
 // n & 3 (T = 2, up to four: columns 4 .. 7 are the same heads for a second tile).
-template <int NG>
+template <int NG, int T>
 struct Q4Query {
   uint32_t b[NG][4];            // B fragments of the two matrix instructions of a group
-  float start[NG][2];           // -8 * sum of the group's elements, in the units of the dot products (2^-24); columns 2c, 2c + 1
+  // -8 * sum of each group's elements, in the units of the dot products (2^-24). T = 1: the B fragment of a product over the
+  // groups, as fp16 and what it leaves (out of that, below 2^-15 of a step of the largest element). T = 2, where a product would
+  // need the scales of two tiles: columns 2c, 2c + 1
+  uint32_t starts[NG > 4 ? 2 : 1];
+  float start[T == 2 ? NG : 1][2];
   float factor[2];              // from the dot products to the base-2 score
+  uint32_t eight[NG];           // A fragments with -8 * 2^-24 in row g
 };
 
 template <int NG, int T, bool BF16>
-__device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, int heads, float scale) {
+__device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* q, int heads, float scale) {
   constexpr int HD = NG * 32;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = T == 1 ? r : r & 3;
   float x[NG][8];
@@ -129,6 +149,7 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, 
   const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 116);
   const float up = __int_as_float((127 + 14 - e) << 23), up16 = up * 0.0625f;
   const float back = __int_as_float((127 + 10 + e) << 23) * scale;           // 2^24 / up
+  float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     float sum = 0.f;
@@ -144,9 +165,23 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG>& f, const uint8_t* q, 
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     sum *= -8.f / 16777216.f;
+    if (T == 1) {
+      if ((g & 3) == c) own[g >> 2] = sum;                                   // k slots 2c, 2c + 1 belong to group c (and c + 4)
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) f.start[g][i] = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * i);   // column 2c + i: lanes 4 (2c + i) ..
+      for (int i = 0; i < 2; ++i) f.start[g][i] = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * i);  // column 2c + i: lanes 4 (2c + i) ..
+    }
   }
+  if (T == 1) {
+#pragma unroll
+    for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
+      const __half hi = __float2half_rn(own[i]);
+      const __half2 both = __halves2half2(hi, __float2half_rn(own[i] - __half2float(hi)));
+      f.starts[i] = *reinterpret_cast<const uint32_t*>(&both);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) f.eight[g] = r == g ? 0x80088008u : 0u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) f.factor[i] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * i);
 }
@@ -197,11 +232,11 @@ struct Q4State {
   }
 };
 
-// T tiles of 16 tokens in shared memory, neighbours in the sequence; `live` tokens belong to the sequence (16 T or more: all),
-// bit j of `gone`: tile T - 1 - j is not there. With T = 2 both tiles go through the same columns' arithmetic at once: columns
+// T tiles of 16 tokens in shared memory, neighbours in the sequence. WHOLE: all of them belong to it; else `live` tokens do, bit
+// j of `gone`: tile T - 1 - j is not there. With T = 2 both tiles go through the same columns' arithmetic at once: columns
 // 0 .. 3 are the heads over the first tile, 4 .. 7 over the second, which a group of at most four heads would leave idle.
-template <int NG, int T>
-__device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG>& f, const uint8_t* tiles, int live, uint32_t gone) {
+template <int NG, int T, bool WHOLE>
+__device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f, const uint8_t* tiles, int live, uint32_t gone) {
   constexpr int NP = NG / 2, TILE = 576 * NG;    // NP: 16-byte pieces per lane of the keys, and of the values
   const int lane = threadIdx.x & 31, r = lane >> 2, second = T == 2 ? (lane >> 1) & 1 : 0;
   // scales of tokens r and r + 8 of this lane's tile: NG fp16 of the keys, NG of the values
@@ -225,6 +260,18 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG>& f, c
   }
   // ---- scores of tokens r, r + 8 and columns 2c, 2c + 1: s[2 j + e]
   float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (T == 1) {                                  // the part of the -8: key scales times `starts`
+    const uint32_t pick = 0x1010u + 0x2222u * (NG == 2 ? lane & 1 : lane & 3);       // scale of group c, twice
+    const uint32_t a0 = __byte_perm(sc[0][0], sc[0][NG == 2 ? 0 : 1], pick), a1 = __byte_perm(sc[1][0], sc[1][NG == 2 ? 0 : 1], pick);
+    if (NG <= 4) {
+      mma_f16_first(s, a0, a1, 0u, 0u, f.starts[0], 0u);
+    } else {
+      const uint32_t pick2 = 0x1010u + 0x2222u * (NG == 6 ? lane & 1 : lane & 3);    // and of group c + 4
+      constexpr int K2 = NG > 4 ? 2 : 0, K3 = NG == 8 ? 3 : K2;
+      mma_f16_first(s, a0, a1, __byte_perm(sc[0][K2], sc[0][K3], pick2), __byte_perm(sc[1][K2], sc[1][K3], pick2), f.starts[0],
+                    f.starts[NG > 4 ? 1 : 0]);
+    }
+  }
   {
     uint32_t kw[T][2 * NG];
 #pragma unroll
@@ -251,13 +298,12 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG>& f, c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float dot = T == 2 && second ? d[T - 1][2 * j + e] : d[0][2 * j + e];
-          s[2 * j + e] = fmaf(ks, dot + f.start[g][e], s[2 * j + e]);
+          s[2 * j + e] = fmaf(ks, T == 2 ? dot + f.start[T == 2 ? g : 0][e] : dot, s[2 * j + e]);
         }
       }
     }
   }
-  if (live < T * kQ4Tile || gone != 0u) {
-    asm volatile("" ::: "memory");               // a branch: nearly all passes skip it
+  if (!WHOLE) {
     const int mine = (gone >> (T - 1 - second) & 1) ? 0 : live - second * kQ4Tile;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -316,8 +362,7 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG>& f, c
   for (int g = 0; g < NG; ++g) {
     const uint32_t b0 = transpose8(pack_f16x2(p[0] * sv[0][g], p[1] * sv[0][g]));
     const uint32_t b1 = transpose8(pack_f16x2(p[2] * sv[1][g], p[3] * sv[1][g]));
-    const uint32_t eight = r == g ? 0x80088008u : 0u;                                  // -8 * 2^-24 in row g
-    mma_f16(st.z, eight, 0u, eight, 0u, b0, b1);
+    { const uint32_t eight = r == g ? 0x80088008u : 0u; mma_f16(st.z, eight, 0u, eight, 0u, b0, b1); }
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const uint32_t mine = T == 1 ? 0xffffffffu : (r >> 2) == t ? 0xffffffffu : 0u;   // the columns of this tile
@@ -495,13 +540,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
       for (int t = 0; t < T; ++t) {
         const int tile = __shfl_sync(0xffffffffu, list, at + t);
         missing = missing * 2 + (tile < 0);
-        if (tile >= 0) {
-          const uint8_t* from = from0 + (size_t)(uint32_t)tile * TILE;
-          const uint32_t to = to0 + stage_in + t * TILE;
-#pragma unroll
-          for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
-          if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
-        }
+        copy_tile<NG>(to0 + stage_in + t * TILE, from0 + (size_t)(uint32_t)max(tile, 0) * TILE, tile >= 0);
       }
       at += T;
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -510,7 +549,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) issue();
 
-    Q4Query<NG> f;
+    Q4Query<NG, T> f;
     Q4State<NG> st;
     int mine = 0;
     const uint8_t* tiles = ring;
@@ -526,7 +565,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
         const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
         if (first) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
         issue();
-        q4_pass<NG, T>(st, f, tiles, live, gone);
+        if (live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
+        else q4_pass<NG, T, false>(st, f, tiles, live, gone);
         tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
       }
       mine = stop;
@@ -610,13 +650,7 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
     for (int t = 0; t < T; ++t) {
       const int tile = __shfl_sync(0xffffffffu, list, (at + t) & 31);
       missing = missing * 2 + (tile < 0);
-      if (tile >= 0) {
-        const uint8_t* from = from0 + (size_t)(uint32_t)tile * TILE;
-        const uint32_t to = to0 + stage_in + t * TILE;
-#pragma unroll
-        for (int i = 0; i < TILE / 512; ++i) copy16(to + i * 512, from + i * 512);
-        if (TILE % 512 != 0 && lane * 16 < TILE % 512) copy16(to + TILE / 512 * 512, from + TILE / 512 * 512);
-      }
+      copy_tile<NG>(to0 + stage_in + t * TILE, from0 + (size_t)(uint32_t)max(tile, 0) * TILE, tile >= 0);
     }
     at += T;
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -628,7 +662,7 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) issue();
   }
-  Q4Query<NG> f;
+  Q4Query<NG, T> f;
   Q4State<NG> st;
   st.clear();
   const uint8_t* tiles = ring;
@@ -638,7 +672,9 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
     const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
     if (pass == warp) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
     issue();
-    q4_pass<NG, T>(st, f, tiles, len - pass * T * kQ4Tile, gone);
+    const int live = len - pass * T * kQ4Tile;
+    if (live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
+    else q4_pass<NG, T, false>(st, f, tiles, live, gone);
     tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -856,24 +892,39 @@ ICB_API int icb_paged_decode_q4_plan(int hd, int per, int dtype, long long units
   return -(int)(need < 1 ? 1 : need < fit ? need : fit);
 }
 
-// q: [rows, hq * hd] 16-bit rows of pitch q_stride (16-byte aligned); pool: num_blocks pages of [hkv][tiles] tiles; row i
-// attends over the first lens[i] tokens of table row seqs[i] (null: i). out: [rows, out_stride], same type. hd 64, 128, 192
-// or 256. plan: as icb_paged_decode_q4_plan gives it; where it is negative, scratch has blocks * 4 * (4 + 2 * min(8, hq / hkv)
-// * (hd + 4)) floats, 16-byte aligned.
-ICB_API int icb_paged_decode_q4(const void* q, long long q_stride, const void* pool, const int* block_table, const int* seqs,
-                                const int* lens, void* out, long long out_stride, void* scratch, int rows, int hq, int hkv,
-                                int hd, int tiles, int max_blocks, int table_rows, int num_blocks, int plan, float scale,
-                                int dtype, void* stream) {
-  if (rows <= 0) return 0;
-  if (hkv < 1 || hq < 1 || hq % hkv || tiles < 1 || plan == 0 || plan > (hd <= 128 ? 16 : 8) || q_stride % 8) return -2;
-  const int slices = (hq / hkv + 7) / 8, blocks = plan < 0 ? -plan : 0;
+// The arguments of icb_paged_decode_q4 come as one record: a caller through ctypes packs it in 0.7 us, where 22 arguments by
+// themselves took 3.4 us of the 9 that a short call takes on the host.
+//   q: [rows, hq * hd] 16-bit rows of pitch q_stride (16-byte aligned); pool: num_blocks pages of [hkv][tiles] tiles; row i
+//   attends over the first lens[i] tokens of table row seqs[i] (null: i). out: [rows, out_stride], same type. hd 64, 128, 192
+//   or 256. plan: as icb_paged_decode_q4_plan gives it; where it is negative, scratch has blocks * 4 * (4 + 2 * min(8, hq / hkv)
+//   * (hd + 4)) floats, 16-byte aligned.
+struct Q4DecodeCall {
+  const uint16_t* q;
+  long long q_stride;
+  const uint8_t* pool;
+  const int *block_table, *seqs, *lens;
+  uint16_t* out;
+  long long out_stride;
+  float* scratch;
+  long long rows, hq, hkv, hd, tiles, max_blocks, table_rows, num_blocks, plan;
+  double scale;
+  long long dtype;
+};
+
+ICB_API int icb_paged_decode_q4(const void* record, void* stream) {
+  Q4DecodeCall c;
+  memcpy(&c, record, sizeof(c));
+  if (c.rows <= 0) return 0;
+  if (c.hkv < 1 || c.hq < 1 || c.hq % c.hkv || c.tiles < 1 || c.plan == 0 || c.plan > (c.hd <= 128 ? 16 : 8) || c.q_stride % 8) return -2;
+  const long long per = c.hq / c.hkv, slices = (per + 7) / 8, blocks = c.plan < 0 ? -c.plan : 0;
   // the numbers of a pool's tiles and of a row's tiles in all units are 32-bit
-  if ((long long)max_blocks * tiles * hkv * slices > 0x7fffffffLL || (long long)max_blocks * tiles > 0x7ffffffLL ||
-      (long long)num_blocks * hkv * tiles > 0x7fffffffLL || (long long)rows * hkv * slices > 0x7fffffffLL)
+  if (c.max_blocks * c.tiles * c.hkv * slices > 0x7fffffffLL || c.max_blocks * c.tiles > 0x7ffffffLL ||
+      c.num_blocks * c.hkv * c.tiles > 0x7fffffffLL || c.rows * c.hkv * slices > 0x7fffffffLL || c.hq > 0x7fffffffLL ||
+      c.table_rows > 0x7fffffffLL || blocks > 0x7fffffffLL)
     return -2;
-  Q4DecodeArgs a{reinterpret_cast<const uint16_t*>(q), q_stride, reinterpret_cast<const uint8_t*>(pool), block_table, seqs,
-                 lens, reinterpret_cast<uint16_t*>(out), out_stride, reinterpret_cast<int4*>(scratch), 0,
-                 reinterpret_cast<float*>(scratch) + (size_t)blocks * kQ4Warps * 4, rows, hq, hkv, slices,
-                 hq / hkv < 8 ? hq / hkv : 8, tiles, max_blocks, table_rows, num_blocks, scale * kLog2e};
-  return q4_variant<true>(hd, hq / hkv, dtype, &a, blocks, plan > 0 ? plan : 0, reinterpret_cast<cudaStream_t>(stream));
+  Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride, reinterpret_cast<int4*>(c.scratch), 0,
+                 c.scratch + (size_t)blocks * kQ4Warps * 4, (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8),
+                 (int)c.tiles, (int)c.max_blocks, (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
+  return q4_variant<true>((int)c.hd, (int)per, (int)c.dtype, &a, (int)blocks, c.plan > 0 ? (int)c.plan : 0,
+                          reinterpret_cast<cudaStream_t>(stream));
 }

@@ -194,6 +194,11 @@ except ImportError:  # pragma: no cover - a build of torch without CUDA
     _raw_stream = None
 
 
+def current_device() -> int:
+    """Index of the current CUDA device."""
+    return torch.cuda.current_device() if _raw_stream is None else _current_device()
+
+
 def stream_ptr():
     if _raw_stream is None or not torch.cuda.is_initialized():
         return torch.cuda.current_stream().cuda_stream

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -19,13 +20,16 @@ from .native import call, dtype_code, ptr, stream_ptr
 P, I, L, F = native.P, native.I, native.L, native.F
 native.register("icb_kv_append", [P, P, P, P, P, I, I, L, L, P])
 native.register("icb_paged_decode", [P, L, P, P, P, P, P, P, I, I, I, I, I, I, F, I, P, P, I, P, I, I, I, P, L])
-native.register("icb_kv_append_q4", [P, P, P, P, L, I, I, I, L, L, L, I, P])
-native.register("icb_kv_read_q4", [P, P, P, P, L, I, I, I, L, I, P])
-native.register("icb_paged_decode_q4", [P, L, P, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, P])
+# these take their arguments as one packed record: see csrc/paged_q4.cu and csrc/paged_q4_decode.cu
+native.register("icb_kv_append_q4", [ctypes.c_char_p, P])
+native.register("icb_kv_read_q4", [ctypes.c_char_p, P])
+native.register("icb_paged_decode_q4", [ctypes.c_char_p, P])
+_ROWS_CALL = struct.Struct("12q").pack
+_DECODE_CALL = struct.Struct("18qdq").pack
 native.register("icb_paged_decode_q4_plan", [I, I, I, L, L])
 native.register("icb_copy_pages", [P, I, P, P, I, P])
 _SMS = None
-_HALF = (torch.bfloat16, torch.float16)
+_HALF = {dt: dtype_code(dt) for dt in (torch.bfloat16, torch.float16)}
 Q4_GROUP = 32                                       # elements that share a scale
 Q4_HEAD_DIMS = (64, 128, 192, 256)
 
@@ -113,8 +117,8 @@ def paged_decode(q: torch.Tensor, k_cache, v_cache, block_table, seq_lens, hq: i
 
 # --------------------------------------------------------------------------- pages
 def _elsewhere(dev: int) -> bool:
-    """Whether a launch for tensors on CUDA device ``dev`` needs another current device."""
-    return dev >= 0 and dev != torch.cuda.current_device()
+    """Whether launches for tensors on CUDA device ``dev`` need another current device."""
+    return dev != native.current_device()
 
 
 def _page_numbers(x, name: str) -> torch.Tensor:
@@ -329,8 +333,8 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slots: to
             kv_append_q4(k, v, pool, slots)
         return
     k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
-    call("icb_kv_append_q4", k.data_ptr(), v.data_ptr(), pool.data_ptr(), slots.data_ptr(), shape[0], hkv, hd, tiles,
-         blocks * tiles * 16, k.stride(0), v.stride(0), dtype_code(dtype), stream_ptr())
+    call("icb_kv_append_q4", _ROWS_CALL(k.data_ptr(), v.data_ptr(), pool.data_ptr(), slots.data_ptr(), shape[0], hkv, hd, tiles,
+                                        blocks * tiles * 16, k.stride(0), v.stride(0), _HALF[dtype]), stream_ptr())
 
 
 def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
@@ -353,8 +357,8 @@ def kv_read_q4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = tor
     k = pool.new_empty((t, hkv * hd), dtype=dtype)
     v = torch.empty_like(k)
     slots = slots.contiguous()
-    call("icb_kv_read_q4", pool.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), t, hkv, hd, tiles,
-         blocks * tiles * 16, dtype_code(dtype), stream_ptr())
+    call("icb_kv_read_q4", _ROWS_CALL(k.data_ptr(), v.data_ptr(), pool.data_ptr(), slots.data_ptr(), t, hkv, hd, tiles,
+                                      blocks * tiles * 16, 0, 0, _HALF[dtype]), stream_ptr())
     return k, v
 
 
@@ -398,7 +402,9 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
         seqs = seqs.contiguous()
     plan, floats = _q4_plan(hd, per, dtype, t * hkv * ((per + 7) // 8), pages * tiles)
     scratch = q.new_empty(floats, dtype=torch.float32) if floats else None
-    call("icb_paged_decode_q4", q.data_ptr(), q.stride(0), pool.data_ptr(), block_table.data_ptr(), ptr(seqs),
-         seq_lens.data_ptr(), out.data_ptr(), out.stride(0), ptr(scratch), t, hq, hkv, hd, tiles, pages, table_rows, blocks,
-         plan, scale, dtype_code(dtype), stream_ptr())
+    call("icb_paged_decode_q4",
+         _DECODE_CALL(q.data_ptr(), q.stride(0), pool.data_ptr(), block_table.data_ptr(),
+                      seqs.data_ptr() if seqs is not None else 0, seq_lens.data_ptr(), out.data_ptr(), out.stride(0),
+                      scratch.data_ptr() if scratch is not None else 0, t, hq, hkv, hd, tiles, pages, table_rows, blocks, plan,
+                      scale, _HALF[dtype]), stream_ptr())
     return out
