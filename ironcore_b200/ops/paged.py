@@ -395,9 +395,9 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return paged_decode_q4(q, pool, block_table, seq_lens, hq, scale, seqs=seqs, out=out)
-    if out is None:
-        out = q.new_empty(shape)
     q, block_table, seq_lens = _rows16(q), block_table.contiguous(), seq_lens.contiguous()
+    if out is None:     # the quicker of the two where rows do not overlap: contiguous rows then too
+        out = torch.empty_like(q) if q.stride(0) >= shape[1] else q.new_empty(shape)
     if seqs is not None:
         seqs = seqs.contiguous()
     plan, floats = _q4_plan(hd, per, dtype, t * hkv * ((per + 7) // 8), pages * tiles)

@@ -208,6 +208,12 @@ def test_attention_calls_of_every_form():
     assert not first[5].any() and not first[6].any()
     for lo in (1, 8, 3):
         _check(wide[:, lo:lo + hq * hd], pool, table, lens, hq, seqs=seqs)
+    # one query for all rows, columns before rows, a single row: as their contiguous copies
+    for x in (wide[:1, :hq * hd].expand(8, -1), wide[:, :hq * hd].t().contiguous().t(), wide[2:3, 8:8 + hq * hd]):
+        n = x.shape[0]
+        got = paged.paged_decode_q4(x, pool, table, lens[:n], hq, seqs=seqs[:n])
+        assert torch.equal(got, paged.paged_decode_q4(x.contiguous(), pool, table, lens[:n], hq, seqs=seqs[:n]))
+        assert got.is_contiguous()
     into = torch.full((8, hq * hd + 3), 9.0, dtype=HF, device="cuda")
     paged.paged_decode_q4(wide[:, :hq * hd], pool, table, lens, hq, seqs=seqs, out=into[:, 1:1 + hq * hd])
     assert torch.equal(into[:, 1:1 + hq * hd], first) and bool((into[:, 0] == 9).all()) and bool((into[:, -2:] == 9).all())
