@@ -77,6 +77,11 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
   return *reinterpret_cast<float2*>(&d);
 }
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return *reinterpret_cast<float2*>(&d);
+}
 
 // N codes (at most 8) of a plain group, lowest nibble first.
 template <int N>
@@ -208,34 +213,34 @@ template <bool BF16>
 __device__ __forceinline__ float2 widen2(uint32_t u) {
   return BF16 ? unpack_bf16x2(u) : __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-// Scale of a group whose W registers are here, the rest in the lanes that differ in the bits OFF1 .. OFF2. The largest element
-// and the largest negated one travel in one register.
-template <bool BF16, int W, int OFF1, int OFF2>
-__device__ __forceinline__ Q4Scale q4_group_of(const uint32_t* u) {
+// (largest element, largest negated element) of W registers.
+template <bool BF16, int W>
+__device__ __forceinline__ uint32_t q4_extremes(const uint32_t* u) {
   uint32_t most = u[0], least = u[0];
 #pragma unroll
   for (int i = 1; i < W; ++i) {
     most = max2<BF16>(most, u[i]);
     least = min2<BF16>(least, u[i]);
   }
-  // (most, -least) of the even and of the odd elements
   least ^= 0x80008000u;
-  uint32_t both = max2<BF16>(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
-#pragma unroll
-  for (int off = OFF1; off <= OFF2; off <<= 1) both = max2<BF16>(both, __shfl_xor_sync(0xffffffffu, both, off));
-  const float2 m = widen2<BF16>(both);
-  return q4_group(m.x, -m.y);
+  return max2<BF16>(__byte_perm(most, least, 0x5410), __byte_perm(most, least, 0x7632));
 }
-// NG fp16 scales at once (p aligned to them).
-template <int NG>
-__device__ __forceinline__ void put_scales(__half* p, const __half (&s)[NG]) {
-  if (NG == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(s);
-  else if (NG == 4) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(s);
-  else {
+// N groups' extremes, each spread over the lanes that differ in the bits OFF, OFF / 2 .. LAST: halving the groups at each step
+// while their number is even leaves q4_owned() of them with every lane, all lanes' work on scales being different.
+__host__ __device__ constexpr int q4_owned(int n, int steps) { return steps == 0 || n % 2 ? n : q4_owned(n / 2, steps - 1); }
+template <bool BF16, int N, int OFF, int LAST>
+__device__ __forceinline__ void q4_gather(uint32_t* m) {
+  constexpr int KEEP = N % 2 ? N : N / 2;
+  const bool up = (threadIdx.x & OFF) != 0;
 #pragma unroll
-    for (int i = 0; i < NG; i += 2) *reinterpret_cast<uint32_t*>(p + i) = *reinterpret_cast<const uint32_t*>(s + i);
+  for (int i = 0; i < KEEP; ++i) {
+    const uint32_t send = N % 2 || up ? m[i] : m[i + N - KEEP], keep = N % 2 || !up ? m[i] : m[i + N - KEEP];
+    m[i] = max2<BF16>(keep, __shfl_xor_sync(0xffffffffu, send, OFF));
   }
+  if constexpr (OFF > LAST) q4_gather<BF16, KEEP, OFF / 2, LAST>(m);
 }
+
+// NG fp16 scales at once (p aligned to them).
 template <int NG>
 __device__ __forceinline__ void get_scales(const __half* p, __half (&s)[NG]) {
   if (NG == 8) *reinterpret_cast<uint4*>(s) = *reinterpret_cast<const uint4*>(p);
@@ -282,84 +287,103 @@ kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restr
                          const long long* __restrict__ slots, long long T, int hkv, int tiles, long long num_slots,
                          long long k_stride, long long v_stride, int per) {
   constexpr int HD = NG * 32, PIECES = (HD / 4 + 31) / 32, DEPTH = 4;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5, j = warp & 1;
+  const int h0 = blockIdx.y * per, h1 = min(hkv, h0 + per);
   const long long first = (long long)blockIdx.x * 16;
   const Q4Window w = q4_window(slots, first, T, num_slots);
+  const uint32_t single = __ballot_sync(0xffffffffu, lane < 16 && w.slot >= 0 && w.slot < num_slots) & ~w.covered & (0x1111u << warp);
+  const long long t0 = first + w.leader, slot0 = __shfl_sync(0xffffffffu, w.slot, w.leader & 15);
+  const bool keys = warp < 2;
+  const int tok = 8 * j + (keys ? r : 2 * c);    // the lane's token, for values the first of two
+  uint8_t* tile = pool + q4_tile_of(slot0, h0, hkv, tiles, 18 * HD);
+  const uint16_t* from = keys ? k + (t0 + tok) * k_stride + h0 * HD + c * 8 : v + (t0 + tok) * v_stride + h0 * HD + r * 4;
 #pragma unroll 1
-  for (int h = blockIdx.y * per; h < min(hkv, (int)(blockIdx.y + 1) * per); ++h) {
+  for (int h = h0; h < h1; ++h, tile += tiles * 18 * HD, from += HD) {
     // rows that go one by one: bit i for row row0 + i, whose slot lane i has; pieces p0 to p1 of them
     long long row0 = first, slot = w.slot;
     uint32_t left = 0;
     int p0 = 0, p1 = HD / 4;
     if (w.leader >= 0) {
-      const long long t0 = first + w.leader, slot0 = __shfl_sync(0xffffffffu, w.slot, w.leader);
-      uint8_t* tile = pool + q4_tile_of(slot0, h, hkv, tiles, 18 * HD);
       __half* scales = reinterpret_cast<__half*>(tile + 16 * HD);
-      const int j = warp & 1;
       uint32_t word[NG];
       bool plain = true;
-      if (warp < 2) {                              // keys: token 8 j + r, elements 32 g + 8 c ..
-        const int tok = 8 * j + r;
-        const uint16_t* from = k + (t0 + tok) * k_stride + h * HD + c * 8;
+      if (keys) {                                // elements 32 g + 8 c .. of a token
+        constexpr int OWN = q4_owned(NG, 2), SHIFT = NG / OWN == 4 ? 0 : 1;
         uint4 u[NG];
+        uint32_t m[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) u[g] = *reinterpret_cast<const uint4*>(from + g * 32);
-        __align__(16) __half row[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const uint32_t x2[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
-          const Q4Scale s = q4_group_of<BF16, 4, 1, 2>(x2);
-          float x[8];
-          widen8<BF16>(u[g], x);
-          word[g] = q4_codes(x, s.inv);
-          row[g] = s.half;
+          m[g] = q4_extremes<BF16, 4>(x2);
+        }
+        q4_gather<BF16, NG, 2, 1>(m);
+        float inv[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+          const float2 x = widen2<BF16>(m[i]);
+          const Q4Scale s = q4_group(x.x, -x.y);
+          inv[i] = s.inv;
           plain &= s.plain;
+          scales[tok * 2 * NG + (c >> SHIFT) * OWN + i] = s.half;
         }
-        put_words<NG>(tile, j * NG, word);
-        if (c == 0) put_scales<NG>(scales + tok * 2 * NG, row);
-        p1 = HD / 8;
-      } else {                                     // values: tokens 8 j + 2 c, + 1, elements 32 g + 4 r ..
-        const int tok = 8 * j + 2 * c;
-        uint2 u[2][NG];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint16_t* from = v + (t0 + tok + e) * v_stride + h * HD + r * 4;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) u[e][g] = *reinterpret_cast<const uint2*>(from + g * 32);
-        }
-        __align__(16) __half row[2][NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          uint32_t both = 0;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t x2[2] = {u[e][g].x, u[e][g].y};
-            const Q4Scale s = q4_group_of<BF16, 2, 4, 16>(x2);
-            const float2 lo = widen2<BF16>(x2[0]), hi = widen2<BF16>(x2[1]);
-            const float x[4] = {lo.x, lo.y, hi.x, hi.y};
-            both |= q4_codes(x, s.inv) << (16 * e);
-            row[e][g] = s.half;
-            plain &= s.plain;
-          }
-          word[g] = both;
+          float x[8];
+          widen8<BF16>(u[g], x);
+          word[g] = q4_codes(x, __shfl_sync(0xffffffffu, inv[g % OWN], 4 * r + (g / OWN << SHIFT)));
         }
-        put_words<NG>(tile + 8 * HD, j * NG, word);
+        put_words<NG>(tile, j * NG, word);
+        p1 = HD / 8;
+      } else {                                   // elements 32 g + 4 r .. of two tokens
+        constexpr int OWN = q4_owned(2 * NG, 3), SHIFT = 2 * NG / OWN == 8 ? 0 : 1;
+        uint2 u[2][NG];
+        uint32_t m[2 * NG];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (r == 0) put_scales<NG>(scales + (tok + e) * 2 * NG + NG, row[e]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) u[e][g] = *reinterpret_cast<const uint2*>(from + e * v_stride + g * 32);
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) {
+          const uint32_t x2[2] = {u[i / NG][i % NG].x, u[i / NG][i % NG].y};
+          m[i] = q4_extremes<BF16, 2>(x2);
+        }
+        q4_gather<BF16, 2 * NG, 16, 4>(m);
+        float inv[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+          const float2 x = widen2<BF16>(m[i]);
+          const Q4Scale s = q4_group(x.x, -x.y);
+          inv[i] = s.inv;
+          plain &= s.plain;
+          const int which = (r >> SHIFT) * OWN + i, e = which >= NG;
+          scales[(tok + e) * 2 * NG + NG + which - e * NG] = s.half;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) word[g] = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) {
+          const uint2& t = u[i / NG][i % NG];
+          const float2 lo = widen2<BF16>(t.x), hi = widen2<BF16>(t.y);
+          const float x[4] = {lo.x, lo.y, hi.x, hi.y};
+          word[i % NG] |= q4_codes(x, __shfl_sync(0xffffffffu, inv[i % OWN], 4 * (i / OWN << SHIFT) + c)) << (16 * (i / NG));
+        }
+        put_words<NG>(tile + 8 * HD, j * NG, word);
         p0 = HD / 8;
       }
-      if (!__all_sync(0xffffffffu, plain)) {       // a group needs the long way: the warp's part takes it, over what it wrote
+      if (!__all_sync(0xffffffffu, plain)) {     // a group needs the long way: the warp's part takes it, over what it wrote
         __syncwarp();
         row0 = t0;
         slot = slot0 + (lane & 15);
         left = 0xffu << (8 * j);
       }
     }
+    if ((left | single) == 0u) continue;
 #pragma unroll 1
-    for (int turn = 0; turn < 2; ++turn) {         // the warp's part once more, then its share of the rows that fill no tile
+    for (int turn = 0; turn < 2; ++turn) {       // the warp's part once more, then its share of the rows that fill no tile
       while (left != 0u) {
-        uint4 u[DEPTH][PIECES];                    // some rows at a time, so that their loads share a wait
+        uint4 u[DEPTH][PIECES];                  // some rows at a time, so that their loads share a wait
         uint32_t rest = left;
 #pragma unroll
         for (int i = 0; i < DEPTH; ++i) {
@@ -368,7 +392,8 @@ kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restr
           for (int p = 0; p < PIECES; ++p) {
             const int piece = p0 + p * 32 + lane;
             u[i][p] = make_uint4(0u, 0u, 0u, 0u);
-            if (row >= 0 && piece < p1) u[i][p] = *reinterpret_cast<const uint4*>(q4_piece_of(k, v, row0 + row, h, piece, HD, k_stride, v_stride));
+            if (row >= 0 && piece < p1)
+              u[i][p] = *reinterpret_cast<const uint4*>(q4_piece_of(k, v, row0 + row, h, piece, HD, k_stride, v_stride));
           }
           rest &= rest - 1;
         }
@@ -389,21 +414,23 @@ kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restr
       slot = w.slot;
       p0 = 0;
       p1 = HD / 4;
-      left = __ballot_sync(0xffffffffu, lane < 16 && slot >= 0 && slot < num_slots) & ~w.covered & (0x1111u << warp);
+      left = single;
     }
   }
 }
 
-// 8 elements from their codes.
+// 4 elements from their codes: a nibble at the bottom of the upper half of 0x43000000 is the float 128 + code.
 template <bool BF16>
 __device__ __forceinline__ uint32_t q4_value2(uint32_t a, uint32_t b, float scale) {
-  // 2^23 + code as a float, less 2^23 + 8
-  const float lo = (__uint_as_float(a | 0x4b000000u) - 8388616.f) * scale, hi = (__uint_as_float(b | 0x4b000000u) - 8388616.f) * scale;
-  return BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+  const float2 n = fadd2(make_float2(__uint_as_float((a & 0xf0000u) | 0x43000000u), __uint_as_float((b & 0xf0000u) | 0x43000000u)),
+                         make_float2(-136.f, -136.f));
+  const float2 x = fmul2(n, make_float2(scale, scale));
+  return BF16 ? pack_bf16x2(x.x, x.y) : pack_f16x2(x.x, x.y);
 }
-template <bool BF16>
-__device__ __forceinline__ uint2 q4_values4(uint32_t codes, float scale) {
-  return make_uint2(q4_value2<BF16>(codes & 15u, codes >> 4 & 15u, scale), q4_value2<BF16>(codes >> 8 & 15u, codes >> 12 & 15u, scale));
+template <bool BF16, int AT>                     // the codes at bits AT .. AT + 15
+__device__ __forceinline__ uint2 q4_values4(uint32_t word, float scale) {
+  return AT == 0 ? make_uint2(q4_value2<BF16>(word << 16, word << 12, scale), q4_value2<BF16>(word << 8, word << 4, scale))
+                 : make_uint2(q4_value2<BF16>(word, word >> 4, scale), q4_value2<BF16>(word >> 8, word >> 12, scale));
 }
 
 struct Q4Piece {
@@ -433,7 +460,7 @@ __device__ __forceinline__ void q4_write_piece(const Q4Piece& x, uint16_t* __res
                                                int h, int piece, int hkv, int hd) {
   const int per = hd / 8;
   const float scale = __half2float(x.scale);
-  const uint2 a = q4_values4<BF16>(x.word & 0xffffu, scale), b = q4_values4<BF16>(x.word >> 16, scale);
+  const uint2 a = q4_values4<BF16, 0>(x.word, scale), b = q4_values4<BF16, 16>(x.word, scale);
   *reinterpret_cast<uint4*>((piece >= per ? v + (piece - per) * 8 : k + piece * 8) + (t * hkv + h) * hd) = make_uint4(a.x, a.y, b.x, b.y);
 }
 
@@ -455,56 +482,57 @@ __global__ void __launch_bounds__(kQ4RowWarps * 32)
 kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __restrict__ slots, uint16_t* __restrict__ k,
                        uint16_t* __restrict__ v, long long T, int hkv, int tiles, long long num_slots, int per) {
   constexpr int HD = NG * 32, PIECES = (HD / 4 + 31) / 32, DEPTH = 4;
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
-  const long long first = (long long)blockIdx.x * 16;
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5, j = warp & 1;
+  const int h0 = blockIdx.y * per, h1 = min(hkv, h0 + per);
+  const long long first = (long long)blockIdx.x * 16, pitch = (long long)hkv * HD;
   const Q4Window w = q4_window(slots, first, T, num_slots);
+  // this warp's share of the rows that fill no tile
+  const uint32_t single = ~w.covered & (first + 16 <= T ? 0xffffu : (1u << (T - first)) - 1u) & (0x1111u << warp);
+  const long long t0 = first + w.leader, slot0 = __shfl_sync(0xffffffffu, w.slot, w.leader & 15);
+  const bool keys = warp < 2;
+  const int tok = 8 * j + (keys ? r : 2 * c);
+  const uint8_t* tile = pool + q4_tile_of(slot0, h0, hkv, tiles, 18 * HD);
+  uint16_t* to = keys ? k + (t0 + tok) * pitch + h0 * HD + c * 8 : v + (t0 + tok) * pitch + h0 * HD + r * 4;
 #pragma unroll 1
-  for (int h = blockIdx.y * per; h < min(hkv, (int)(blockIdx.y + 1) * per); ++h) {
+  for (int h = h0; h < h1; ++h, tile += tiles * 18 * HD, to += HD) {
     if (w.leader >= 0) {
-      const long long t0 = first + w.leader, pitch = (long long)hkv * HD;
-      const uint8_t* tile = pool + q4_tile_of(__shfl_sync(0xffffffffu, w.slot, w.leader), h, hkv, tiles, 18 * HD);
-      const __half* scales = reinterpret_cast<const __half*>(tile + 16 * HD);
-      const int j = warp & 1;
+      const __half* scales = reinterpret_cast<const __half*>(tile + 16 * HD) + tok * 2 * NG;
       uint32_t word[NG];
-      if (warp < 2) {                              // keys: token 8 j + r, elements 32 g + 8 c ..
-        const int tok = 8 * j + r;
+      if (keys) {                                // elements 32 g + 8 c .. of a token
         __align__(16) __half row[NG];
         get_words<NG>(tile, j * NG, word);
-        get_scales<NG>(scales + tok * 2 * NG, row);
-        uint16_t* to = k + (t0 + tok) * pitch + h * HD + c * 8;
+        get_scales<NG>(scales, row);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float scale = __half2float(row[g]);
-          const uint2 a = q4_values4<BF16>(word[g] & 0xffffu, scale), b = q4_values4<BF16>(word[g] >> 16, scale);
+          const uint2 a = q4_values4<BF16, 0>(word[g], scale), b = q4_values4<BF16, 16>(word[g], scale);
           *reinterpret_cast<uint4*>(to + g * 32) = make_uint4(a.x, a.y, b.x, b.y);
         }
-      } else {                                     // values: tokens 8 j + 2 c, + 1, elements 32 g + 4 r ..
-        const int tok = 8 * j + 2 * c;
+      } else {                                   // elements 32 g + 4 r .. of two tokens
         __align__(16) __half row[2][NG];
         get_words<NG>(tile + 8 * HD, j * NG, word);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) get_scales<NG>(scales + (tok + e) * 2 * NG + NG, row[e]);
+        for (int e = 0; e < 2; ++e) get_scales<NG>(scales + e * 2 * NG + NG, row[e]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint16_t* to = v + (t0 + tok + e) * pitch + h * HD + r * 4;
-#pragma unroll
-          for (int g = 0; g < NG; ++g)
-            *reinterpret_cast<uint2*>(to + g * 32) = q4_values4<BF16>(e ? word[g] >> 16 : word[g] & 0xffffu, __half2float(row[e][g]));
+        for (int g = 0; g < NG; ++g) {
+          *reinterpret_cast<uint2*>(to + g * 32) = q4_values4<BF16, 0>(word[g], __half2float(row[0][g]));
+          *reinterpret_cast<uint2*>(to + pitch + g * 32) = q4_values4<BF16, 16>(word[g], __half2float(row[1][g]));
         }
       }
     }
-    // this warp's share of the rows that fill no tile, some at a time so that their loads share a wait
-    uint32_t left = ~w.covered & (first + 16 <= T ? 0xffffu : (1u << (T - first)) - 1u) & (0x1111u << warp);
+    uint32_t left = single;
     while (left != 0u) {
-      Q4Piece x[DEPTH][PIECES];
+      Q4Piece x[DEPTH][PIECES];                  // some rows at a time, so that their loads share a wait
       uint32_t rest = left;
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i) {
         const int row = __ffs(rest) - 1;
         const long long slot = __shfl_sync(0xffffffffu, w.slot, max(row, 0));
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-          x[i][p] = q4_get_piece(pool, slot, h, p * 32 + lane, row >= 0 && p * 32 + lane < HD / 4 && slot >= 0 && slot < num_slots, hkv, HD, tiles);
+        for (int p = 0; p < PIECES; ++p) {
+          const int piece = p * 32 + lane;
+          x[i][p] = q4_get_piece(pool, slot, h, piece, row >= 0 && piece < HD / 4 && slot >= 0 && slot < num_slots, hkv, HD, tiles);
+        }
         rest &= rest - 1;
       }
 #pragma unroll
