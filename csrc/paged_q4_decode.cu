@@ -483,7 +483,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
       at[i] = min(plan.total, (worker + i) * plan.per);
       if (at[i] == plan.total) continue;
       const int row = plan_rows[warp + i], len = q4_len(a, row), n = q4_count(len);
-      const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]), unit = into / (uint32_t)n, off = into - unit * n;
+      const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]), unit = min(into / (uint32_t)max(n, 1), (uint32_t)plan.units - 1);
+      const uint32_t off = into - unit * n;
       now.row = row;
       now.unit = unit;
       now.len = len;
@@ -519,18 +520,19 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
         entered = false;
       }
       const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices;
+      const int row = min(ahead.row, a.rows - 1);          // lengths that change under the call must not lead out of bounds
       if (!entered) {                                      // the unit's query rows travel with its first tile
         const int g0 = (ahead.unit - kvh * a.slices) * 8, pieces = min(COLUMNS, group - g0) * (HD / 8);
-        const uint16_t* q = a.q + (size_t)ahead.row * a.q_stride + (size_t)(kvh * group + g0) * HD;
+        const uint16_t* q = a.q + (size_t)row * a.q_stride + (size_t)(kvh * group + g0) * HD;
         for (int i = lane; i < pieces; i += 32) copy16(to0 + stage_in + T * TILE + (i - lane) * 16, q + i * 8);
         entered = true;
       }
       filled = min(32, min(ahead.end, count) - fetched);
       if (lane < filled) {
-        const int seq = a.seqs != nullptr ? a.seqs[ahead.row] : ahead.row;
-        const int t = fetched + lane - ahead.begin, page = a.tiles == 1 ? t : t / a.tiles;
+        const int seq = a.seqs != nullptr ? max(0, min(a.seqs[row], a.table_rows - 1)) : row;
+        const int t = fetched + lane - ahead.begin, page = min(a.tiles == 1 ? t : t / a.tiles, a.max_blocks - 1);
         const int block = a.block_table[(size_t)seq * a.max_blocks + page];
-        if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + (t - page * a.tiles);
+        if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + min(t - page * a.tiles, a.tiles - 1);
       }
       fetched += filled;
     };
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
           const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
           const float4 o = make_float4((st.o[g][0][e] + z) * by, fmaf(st.o[g][0][2 + e], 0.0625f, z) * by,
                                        (st.o[g][1][e] + z) * by, fmaf(st.o[g][1][2 + e], 0.0625f, z) * by);
-          if (h >= heads) continue;
+          if (h >= heads || now.row >= a.rows) continue;
           if (whole) q4_store4<BF16>(a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + 32 * g + 4 * r, o.x, o.y, o.z, o.w);
           else *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) = o;
         }
@@ -597,7 +599,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
       }
       if (begins) {
         owner = whole ? make_int4(-1, 0, 0, 0) : make_int4(now.row, now.unit, worker, (int)((start + now.end - 1) / plan.per));
-        if (a.by_unit && lane == 0) a.owner[(size_t)now.row * plan.units + now.unit] = owner;
+        if (a.by_unit && lane == 0 && now.row < a.rows) a.owner[(size_t)now.row * plan.units + now.unit] = owner;
       }
       if (now.end >= count) break;
       now.next(a, plan.units);

@@ -153,9 +153,9 @@ def copy_pages(pools: Union[torch.Tensor, Sequence[torch.Tensor]], src, dst) -> 
         if t.get_device() != dev:
             raise ValueError("the pools must be on one device")
         if t.numel():
-            size, strides = t.element_size(), t.stride()
-            records += (t.data_ptr(), t.shape[0] if stacked else 1, strides[0] * size if stacked else 0, t.shape[lead],
-                        strides[lead] * size)
+            layers, pages = (t.shape[0] if stacked else 1), t.shape[lead]
+            page = t.numel() // (layers * pages) * t.element_size()      # strides of single layers and pages say nothing
+            records += (t.data_ptr(), layers, pages * page, pages, page)
     if src.get_device() >= 0 or dst.get_device() >= 0:
         if not src.get_device() == dst.get_device() == dev or not src.dtype == dst.dtype == torch.int32:
             raise ValueError("page numbers on the device must be int32, both on the pools' device")

@@ -102,17 +102,26 @@ def test_append_extreme_groups_among_many_rows(dtype):
         assert torch.equal(x.cpu().nan_to_num(), y.nan_to_num()) and torch.equal(x.cpu().isnan(), y.isnan())
 
 
+def _widened(table, bs):
+    """The table with room for 20000 tokens, which sends a call to the kernel that cuts all tiles into ranges."""
+    return torch.cat((table, torch.full((table.shape[0], 20000 // bs), -1, dtype=torch.int32, device=table.device)), 1)
+
+
 def _check(q, pool, table, lens, hq, scale=None, **kw):
+    """Both kernels, by the width of the table; the result of the first."""
     from ironcore_b200.ops import paged
 
-    hd = pool.shape[3] // 18
-    out = paged.paged_decode_q4(q, pool, table, lens, hq, scale, **kw)
+    hd, bs = pool.shape[3] // 18, 16 * pool.shape[2]
     want, tol = O.attention(q.cpu(), *O.decoded(pool), table.cpu(), lens.cpu(), hq, scale or O.scale_of(hd),
                             kw["seqs"].cpu() if "seqs" in kw else None)
-    off = (out.cpu().double() - want).abs()
-    assert bool(torch.isfinite(out).all())
-    assert bool((off <= tol).all()), f"{float((off / tol).max()):.2f} of the tolerance"
-    return out
+    outs = []
+    for t in (table, _widened(table, bs)):
+        out = paged.paged_decode_q4(q, pool, t, lens, hq, scale, **kw)
+        off = (out.cpu().double() - want).abs()
+        assert bool(torch.isfinite(out).all())
+        assert bool((off <= tol).all()), f"{float((off / tol).max()):.2f} of the tolerance"
+        outs.append(out)
+    return outs[0]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -124,6 +133,15 @@ def test_attention(hq, hkv, hd, bs, dtype):
     q = (2 * torch.randn((10, (hq + 2 * hkv) * hd), generator=torch.Generator().manual_seed(1))).to(dtype).cuda()[:, :hq * hd]
     out = _check(q, pool, table, lens, hq)
     assert not out[1].any()
+
+
+def test_attention_over_many_rows():
+    """More (row, head) pairs than warps on the GPU, some rows empty."""
+    g = torch.Generator().manual_seed(0)
+    lens = [0 if x < 20 else x - 19 for x in torch.randint(0, 220, (304,), generator=g).tolist()]
+    pool, table, lens = O.cache(lens, 8, 128, 16, BF, seed=11, device="cuda")
+    q = torch.randn((304, 8 * 128), generator=g).to(BF).cuda()
+    _check(q, pool, table, lens, 8)
 
 
 @pytest.mark.parametrize("spread", [False, True])
@@ -175,10 +193,11 @@ def test_attention_over_stale_pages():
     q = torch.randn((5, 4 * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
     from ironcore_b200.ops import paged
 
-    out = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)
     k, v = O.decoded(pool)
     want, tol = O.attention(q.cpu(), k.nan_to_num(), v.nan_to_num(), table, dev_lens, 4, O.scale_of(hd))
-    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+    for t in (_widened(table, bs), table):
+        out = paged.paged_decode_q4(q, pool.cuda(), t.cuda(), dev_lens.cuda(), 4)
+        assert bool(((out.cpu().double() - want).abs() <= tol).all())
     # a NaN among the tokens does reach its sequence, and no other
     row = pool[table[1, 0], 0, 0, 16 * hd:].view(torch.float16)
     row[0] = float("nan")
@@ -186,8 +205,10 @@ def test_attention_over_stale_pages():
     assert again[1, :2 * hd].isnan().all() and torch.equal(again[[0, 2, 3, 4]], out[[0, 2, 3, 4]])
     assert torch.equal(again[1, 2 * hd:], out[1, 2 * hd:])
     pool[table[0, 0], 1, 0, 16 * hd:16 * hd + 2] = torch.tensor([float("nan")], dtype=HF).view(torch.uint8)
-    again = paged.paged_decode_q4(q, pool.cuda(), table.cuda(), dev_lens.cuda(), 4)          # the only token of a sequence
-    assert again[0, 2 * hd:].isnan().all() and torch.equal(again[0, :2 * hd], out[0, :2 * hd])
+    for t in (_widened(table, bs), table):
+        again = paged.paged_decode_q4(q, pool.cuda(), t.cuda(), dev_lens.cuda(), 4)          # the only token of a sequence
+        assert again[0, 2 * hd:].isnan().all() and bool(again[0, :2 * hd].isfinite().all())
+    assert torch.equal(again[0, :2 * hd], out[0, :2 * hd])
 
 
 def test_attention_calls_of_every_form():
@@ -199,12 +220,15 @@ def test_attention_calls_of_every_form():
     pool, table, _ = O.cache([100, 60, 90], hkv, hd, bs, HF, seed=4)
     table[1, 1], table[2, 0] = -1, pool.shape[0]
     seqs = torch.tensor([2, 0, 0, 0, 1, 3, -1, 0], dtype=torch.int32).cuda()
-    lens = torch.tensor([90, 100, 1, 50, 60, 9, 9, 10 ** 9], dtype=torch.int32).cuda()
+    lens = torch.tensor([90, 100, 1, 50, 60, 9, 9, 112], dtype=torch.int32).cuda()
     assert table.shape[1] * bs == 112
     table[0, 6] = table[0, 5]                               # the whole row of the table holds pages
     wide = torch.randn((8, hq * hd + 24), generator=torch.Generator().manual_seed(1)).to(HF).cuda()
     pool, table = pool.cuda(), table.cuda()
     first = _check(wide[:, :hq * hd], pool, table, lens, hq, seqs=seqs)
+    beyond = lens.clone()
+    beyond[7] = 10 ** 9                                     # as many as the table has
+    assert torch.equal(paged.paged_decode_q4(wide[:, :hq * hd], pool, table, beyond, hq, seqs=seqs), first)
     assert not first[5].any() and not first[6].any()
     for lo in (1, 8, 3):
         _check(wide[:, lo:lo + hq * hd], pool, table, lens, hq, seqs=seqs)
@@ -227,24 +251,26 @@ def test_attention_is_reproducible_and_runs_on_other_streams():
 
     pool, table, lens = O.cache([1500, 700, 3, 0, 999], 4, 128, 16, BF, seed=6, device="cuda")
     q = torch.randn((5, 16 * 128), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
-    first = paged.paged_decode_q4(q, pool, table, lens, 16)
-    torch.cuda.synchronize()
-    streams = [torch.cuda.Stream() for _ in range(2)]
-    outs = []
-    for i in range(6):
-        with torch.cuda.stream(streams[i % 2]):
-            outs.append(paged.paged_decode_q4(q, pool, table, lens, 16))
-    torch.cuda.synchronize()
-    assert all(torch.equal(o, first) for o in outs)
+    for table in (table, _widened(table, 16)):
+        first = paged.paged_decode_q4(q, pool, table, lens, 16)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        outs = []
+        for i in range(6):
+            with torch.cuda.stream(streams[i % 2]):
+                outs.append(paged.paged_decode_q4(q, pool, table, lens, 16))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, first) for o in outs)
 
 
 def test_attention_in_graphs():
-    """Two captured calls that share nothing, replayed in turn with lengths that change between replays."""
+    """Captured calls that share nothing, replayed in turn with lengths that change between replays."""
     from ironcore_b200.ops import paged
 
     sets = []
-    for seed, hd in ((7, 128), (8, 64)):
+    for seed, hd, wide in ((7, 128, False), (8, 64, False), (9, 128, True), (10, 64, True)):
         pool, table, lens = O.cache([800, 50, 300], 2, hd, 16, BF, seed=seed, device="cuda")
+        table = _widened(table, 16) if wide else table
         q = torch.randn((3, 8 * hd), generator=torch.Generator().manual_seed(seed)).to(BF).cuda()
         paged.paged_decode_q4(q, pool, table, lens, 8)
         torch.cuda.synchronize()
@@ -312,6 +338,9 @@ def test_copy_pages_kernel():
                      torch.tensor([0, 1, 20, 2, 19], dtype=torch.int32).cuda())
     stack[:, [0, 19]] = stack[:, [4, 6]]
     assert torch.equal(stack, got.cpu())
+    one = torch.zeros(4000, dtype=torch.uint8, device="cuda").as_strided((1, 5), (3995, 1))     # a page by itself, an odd stride
+    assert one.is_contiguous()
+    paged.copy_pages([one], torch.zeros(1, dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda())
     views = torch.zeros((9, 5), dtype=torch.uint8, device="cuda").view(-1)[1:41].view(8, 5)      # odd addresses
     views[2] = torch.arange(5)
     paged.copy_pages([views], [2], [7])
