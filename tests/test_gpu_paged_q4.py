@@ -351,6 +351,36 @@ def test_copy_pages_kernel():
         paged.copy_pages(got, torch.tensor([4], dtype=torch.int32).cuda(), [0])
 
 
+def test_layer_caches_fork_rows_and_states():
+    from ironcore_b200.layers.mixer import CacheSpec
+    from ironcore_b200.rl import BlockKVCache, LayerCache
+
+    spec = CacheSpec(rows={"k": 24, "v": 8}, states={"s": ((3, 5), torch.float32), "t": ((7,), None), "u": ((1,), None)})
+    c = LayerCache([spec, spec], max_seqs=5, max_seq_len=64, device="cuda")
+    b = BlockKVCache(3, 2, 64, 20, 16, 5, 64)
+    pos = torch.arange(19, device="cuda")
+    for cache in (c, b):
+        a = cache.acquire()
+        cache.reserve(a, 19)
+        cache.advance(a, 19)
+    for t in (*c.rows[0].values(), *c.rows[1].values(), *c.states[0].values(), *c.states[1].values(), *b.k, *b.v):
+        t.normal_()
+    before = [t.clone() for run in c.states for t in run.values()]
+    forks, others = c.fork(a, 2), b.fork(a, 2)
+    for i in forks:
+        for run in c.rows:
+            for t in run.values():
+                assert torch.equal(t[c.slots_for(torch.full_like(pos, i), pos)], t[c.slots_for(torch.full_like(pos, a), pos)])
+    for t, old in zip((t for run in c.states for t in run.values()), before):
+        want = old.clone()
+        want[forks] = old[a]
+        assert torch.equal(t, want)
+    for i in others:
+        for t in b.k + b.v:
+            t = t.view(-1, 128)
+            assert torch.equal(t[b.slots_for(torch.full_like(pos, i), pos)], t[b.slots_for(torch.full_like(pos, a), pos)])
+
+
 def test_refusals_on_the_gpu():
     from ironcore_b200.ops import paged
 

@@ -311,3 +311,51 @@ def test_layer_caches_fork_rows_and_states():
         assert torch.equal(rows[0], rows[1]) and torch.equal(rows[0], rows[2])
     for name in ("s", "t"):
         assert torch.equal(c.states[0][name][a], c.states[0][name][b]) and torch.equal(c.states[0][name][a], c.states[0][name][d])
+
+
+@pytest.mark.parametrize("family", ["tetepel", "kedavik"])
+def test_residual_stream_models_fork_prompts(family):
+    """Caches of rows and fixed-size states: forked prompts go on as the prompt run by itself, windows included."""
+    import kedavik_cases as K
+    import tetepel_cases as T
+
+    if family == "tetepel":
+        C, cfg = T, T.config([T.layer(window=5), T.layer(heads=2, window=11, ff=None)], streams=3, width=24)
+        w = T.weights(cfg)
+    else:
+        C, cfg = K, K.config([K.mamba(), K.pair(chunk=9)])
+        w = K.weights(cfg)
+    model, c = C.build(cfg, w)
+    eng = T.engine(model, c, max_seqs=6)
+    prompts = [T.tokens(cfg, n, n) for n in (7, 16, 19)]
+    alone, _ = eng.generate(prompts, 20, temperature=0.0)
+    got, _ = eng.generate(prompts, 20, temperature=0.0, samples=3)
+    assert got == [t for t in alone for _ in range(3)]
+    assert eng.cache.free_blocks == eng.cache.num_blocks
+    c.rl.kv_cache_bits = 4
+    with pytest.raises(ValueError):
+        T.engine(model, c)
+
+
+@pytest.mark.parametrize("bits,share", [(16, True), (4, False), (4, True)])
+def test_grpo_on_shared_prompts_and_four_bits(bits, share):
+    from ironcore_b200.config import validate_config
+    from ironcore_b200.parallel import mesh
+    from ironcore_b200.rl.trainer import GRPOTrainer
+
+    mesh.destroy_model_parallel()
+    cfg = tiny_config("llama", max_seq_len=48, max_position_embeddings=48, head_dim=64)
+    cfg.trainer.use_flash_attn = False
+    cfg.rl(num_prompts=2, prompt_len=19, group_size=4, max_new_tokens=8, reward_vocab_subset=64, kv_cache_bits=bits,
+           share_prompts=share)
+    cfg.trainer(micro_batch_size=4, train_batch_size=4, gradient_accumulation_steps=None)
+    cfg.operation.train_steps = 1
+    validate_config(cfg)
+    tr = GRPOTrainer(cfg)
+    batch = tr.rollout()
+    assert batch["tokens"].shape == (8, 27) and batch["logp_old"].shape == (8, 8)
+    for i in range(0, 8, 4):
+        assert bool((batch["tokens"][i:i + 4, :19] == batch["tokens"][i, :19]).all())
+    st = tr.policy_update(batch)
+    # the cache's rounding reaches the sampled tokens' log-probs, no more
+    assert abs(st["ratio_mean"] - 1.0) < (1e-3 if bits == 16 else 0.2)
