@@ -18,6 +18,16 @@
 //     magnitude. Relative error 2^-11 down to 2^-26 of the largest contribution; sums, maxima and p itself stay in fp32.
 // Tokens outside the sequence get probability and value scale zero by selection, so nothing stale in a page (NaN scales
 // included) reaches a result. A page number outside the pool counts as a page outside the sequence.
+//
+// Two kernels. One block per (row, slice of heads) where the table is narrow (q4_unit_warps); else all tiles of the call in one
+// line, cut evenly over the warps that the GPU holds, and a second kernel that joins the parts (Q4Plan).
+//
+// Bounds. The bytes are 4.5 bits an element, each read once: at the copy bandwidth an SM gets a tile of 2304 bytes in about
+// 100 clocks, in which its four schedulers can issue 400 instructions; a tile takes about 300, of them 80 to unpack 4096 codes
+// and 21 matrix instructions (0.27 of their pipe). With 128 registers a thread, 16 warps on an SM issue 0.55 of the slots: the
+// kernels are held by the latencies of dependent instructions, not by memory. Measured in a row over inputs larger than L2: 512
+// rows of 768 tokens, 12 heads on 2 of 128: 31.5 us, 0.55 of the copy bandwidth; 4 rows of 100000, 32 on 8: 89 us, 0.79; 8 rows
+// of 4000, 32 on 32: 33 us, 0.68; 33 rows of 700, 12 on 12 of 64: 10.4 us.
 #include <string.h>
 
 #include "host_common.h"
@@ -233,10 +243,12 @@ struct Q4State {
 };
 
 // T tiles of 16 tokens in shared memory, neighbours in the sequence. WHOLE: all of them belong to it; else `live` tokens do, bit
-// j of `gone`: tile T - 1 - j is not there. With T = 2 both tiles go through the same columns' arithmetic at once: columns
+// j of `gone`: tile T - 1 - j is not there. (Heads over 128 always go the second way: another copy of their code costs more than
+// the masks, 64 rows of 1000 tokens with heads of 256 take 16.6 us with it and 14.6 without.) With T = 2 both tiles go through the same columns' arithmetic at once: columns
 // 0 .. 3 are the heads over the first tile, 4 .. 7 over the second, which a group of at most four heads would leave idle.
 template <int NG, int T, bool WHOLE>
-__device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f, const uint8_t* tiles, int live, uint32_t gone) {
+__device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f, const uint8_t* tiles, int live,
+                                        uint32_t gone) {
   constexpr int NP = NG / 2, TILE = 576 * NG;    // NP: 16-byte pieces per lane of the keys, and of the values
   const int lane = threadIdx.x & 31, r = lane >> 2, second = T == 2 ? (lane >> 1) & 1 : 0;
   // scales of tokens r and r + 8 of this lane's tile: NG fp16 of the keys, NG of the values
@@ -262,7 +274,8 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (T == 1) {                                  // the part of the -8: key scales times `starts`
     const uint32_t pick = 0x1010u + 0x2222u * (NG == 2 ? lane & 1 : lane & 3);       // scale of group c, twice
-    const uint32_t a0 = __byte_perm(sc[0][0], sc[0][NG == 2 ? 0 : 1], pick), a1 = __byte_perm(sc[1][0], sc[1][NG == 2 ? 0 : 1], pick);
+    const uint32_t a0 = __byte_perm(sc[0][0], sc[0][NG == 2 ? 0 : 1], pick);
+    const uint32_t a1 = __byte_perm(sc[1][0], sc[1][NG == 2 ? 0 : 1], pick);
     if (NG <= 4) {
       mma_f16_first(s, a0, a1, 0u, 0u, f.starts[0], 0u);
     } else {
@@ -461,7 +474,8 @@ template <int NG, int T> __host__ __device__ constexpr int q4_smem() { return kQ
 // unit's query rows, filled by asynchronous copies that run ahead across units. A unit that lies within the range is finished
 // from registers; parts of others go to `part` for the kernel below.
 template <int NG, int T, bool BF16>
-__global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
+__global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2)
+paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
   constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = q4_stage<NG, T>(), STAGES = q4_stages<NG, T>(), REC = HD + 4;
   constexpr int COLUMNS = 8 / T;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -483,7 +497,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
       at[i] = min(plan.total, (worker + i) * plan.per);
       if (at[i] == plan.total) continue;
       const int row = plan_rows[warp + i], len = q4_len(a, row), n = q4_count(len);
-      const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]), unit = min(into / (uint32_t)max(n, 1), (uint32_t)plan.units - 1);
+      const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]);
+      const uint32_t unit = min(into / (uint32_t)max(n, 1), (uint32_t)plan.units - 1);
       const uint32_t off = into - unit * n;
       now.row = row;
       now.unit = unit;
@@ -532,7 +547,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
         const int seq = a.seqs != nullptr ? max(0, min(a.seqs[row], a.table_rows - 1)) : row;
         const int t = fetched + lane - ahead.begin, page = min(a.tiles == 1 ? t : t / a.tiles, a.max_blocks - 1);
         const int block = a.block_table[(size_t)seq * a.max_blocks + page];
-        if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + min(t - page * a.tiles, a.tiles - 1);
+        if ((uint32_t)block < (uint32_t)a.num_blocks)
+          list = (block * a.hkv + kvh) * a.tiles + min(t - page * a.tiles, a.tiles - 1);
       }
       fetched += filled;
     };
@@ -567,7 +583,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
         const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
         if (first) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
         issue();
-        if (live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
+        if (NG <= 4 && live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
         else q4_pass<NG, T, false>(st, f, tiles, live, gone);
         tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
       }
@@ -592,7 +608,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG <= 2 ? 6 : NG <= 4 ? 4 : 2) pag
           const float4 o = make_float4((st.o[g][0][e] + z) * by, fmaf(st.o[g][0][2 + e], 0.0625f, z) * by,
                                        (st.o[g][1][e] + z) * by, fmaf(st.o[g][1][2 + e], 0.0625f, z) * by);
           if (h >= heads || now.row >= a.rows) continue;
-          if (whole) q4_store4<BF16>(a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + 32 * g + 4 * r, o.x, o.y, o.z, o.w);
+          uint16_t* to = a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + 32 * g + 4 * r;
+          if (whole) q4_store4<BF16>(to, o.x, o.y, o.z, o.w);
           else *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) = o;
         }
         if (!whole && h < heads && r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
@@ -624,7 +641,8 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
   constexpr int HD = NG * 32, TILE = 576 * NG, STAGE = q4_stage<NG, T>(), STAGES = q4_stages<NG, T>(), REC = HD + 4;
   constexpr int COLUMNS = 8 / T;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int warps = blockDim.x >> 5, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warps = blockDim.x >> 5, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int units = a.hkv * a.slices, row = blockIdx.x / units, unit = blockIdx.x - row * units, group = a.hq / a.hkv;
   const int kvh = a.slices == 1 ? unit : unit / a.slices, g0 = (unit - kvh * a.slices) * 8;
   const int heads = min(COLUMNS, group - g0), head0 = kvh * group + g0;
@@ -633,15 +651,15 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
   uint8_t* ring = smem + warp * STAGES * STAGE;
   const uint32_t to0 = smem_u32(ring) + lane * 16;
   const uint8_t* from0 = a.pool + lane * 16;
-  const int* pages = a.block_table + (size_t)(a.seqs != nullptr ? max(0, min(a.seqs[row], a.table_rows - 1)) : row) * a.max_blocks;
+  const int seq = a.seqs != nullptr ? max(0, min(a.seqs[row], a.table_rows - 1)) : row;
+  const int* pages = a.block_table + (size_t)seq * a.max_blocks;
   int listed = 0, list = -1;
   auto refill = [&]() {
     const int i = listed + lane, t = (warp + i / T * warps) * T + i % T;
-    list = -1;
-    if (t < n) {
-      const int page = a.tiles == 1 ? t : t / a.tiles, block = pages[page];
-      if ((uint32_t)block < (uint32_t)a.num_blocks) list = (block * a.hkv + kvh) * a.tiles + (t - page * a.tiles);
-    }
+    const int page = a.tiles == 1 ? t : t / a.tiles;
+    // read whether the row has the tile or not: the first of these does not wait for the row's length
+    const int block = a.max_blocks > 0 ? pages[min(page, a.max_blocks - 1)] : -1;
+    list = t < n && (uint32_t)block < (uint32_t)a.num_blocks ? (block * a.hkv + kvh) * a.tiles + (t - page * a.tiles) : -1;
     listed += 32;
   };
   int at = 0;
@@ -675,7 +693,7 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
     if (pass == warp) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
     issue();
     const int live = len - pass * T * kQ4Tile;
-    if (live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
+    if (NG <= 4 && live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
     else q4_pass<NG, T, false>(st, f, tiles, live, gone);
     tiles = tiles == ring + (STAGES - 1) * STAGE ? ring : tiles + STAGE;
   }
@@ -705,7 +723,9 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
     const float* rec = records + h * REC;
     float top = kQ4None, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) top = fmaxf(top, rec[p * COLUMNS * REC + HD]);
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
       const float* x = rec + p * COLUMNS * REC;
       const float by = exp2_fast(x[HD] - top);
@@ -714,7 +734,8 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
       acc.x += o.x * by; acc.y += o.y * by; acc.z += o.z * by; acc.w += o.w * by;
     }
     const float by = sum == 0.f ? 0.f : 16777216.f / sum;
-    q4_store4<BF16>(a.out + (size_t)row * a.out_stride + (size_t)(head0 + h) * HD + d, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
+    uint16_t* to = a.out + (size_t)row * a.out_stride + (size_t)(head0 + h) * HD + d;
+    q4_store4<BF16>(to, acc.x * by, acc.y * by, acc.z * by, acc.w * by);
   }
 }
 
@@ -724,7 +745,8 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
 constexpr int kQ4MergeThreads = 256;
 
 template <int NG, bool BF16, bool SPREAD>
-__global__ void __launch_bounds__(kQ4MergeThreads) paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long tasks) {
+__global__ void __launch_bounds__(kQ4MergeThreads)
+paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long tasks) {
   constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4MergeThreads / LANES, DEPTH = 8;
   __shared__ __align__(16) float sm_o[SPREAD ? SETS : 1][HD];
   __shared__ float sm_m[SETS], sm_l[SETS];
@@ -825,12 +847,14 @@ static int q4_unit_warps(int hd, long long units, long long tiles) {
 template <int NG, int T, bool BF16>
 static int launch_q4_units(const Q4DecodeArgs& a, int warps, long long units, cudaStream_t st) {
   auto k = paged_decode_q4_unit_kernel<NG, T, BF16>;
-  constexpr int ring = q4_stages<NG, T>() * q4_stage<NG, T>(), record = 8 * (NG * 32 + 4) * 4, each = ring > record ? ring : record;
+  constexpr int ring = q4_stages<NG, T>() * q4_stage<NG, T>(), record = 8 * (NG * 32 + 4) * 4;
+  constexpr int each = ring > record ? ring : record;
   static int ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (NG <= 4 ? 16 : 8) * each) != cudaSuccess) return -5;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (NG <= 4 ? 16 : 8) * each) != cudaSuccess)
+      return -5;
     ready[dev] = 1;
   }
   k<<<(unsigned)units, warps * 32, warps * each, st>>>(a);
@@ -862,8 +886,9 @@ static int launch_q4_decode(Q4DecodeArgs& a, int blocks, cudaStream_t st) {
   return check_launch("paged_decode_q4");
 }
 
-// What a call needs of a variant: blocks of the kernel for ranges that fit the GPU (run false), or the call itself. T = 2 where at most four query heads
-// share a kv head: at 32 heads on 8, T = 1 leaves half of the columns idle.
+// What a call needs of a variant: blocks of the kernel for ranges that fit the GPU (RUN false), or the call itself. T = 2 where
+// at most four query heads share a kv head, whose passes over one tile would leave half of the columns idle: 4 rows of 100000
+// tokens, 32 heads on 8, took 112 us with T = 1 and 107 with T = 2 in the same state of the rest.
 template <bool RUN>
 static int q4_variant(int hd, int per, int dtype, Q4DecodeArgs* a, int blocks, int warps, cudaStream_t st) {
 #define ICB_Q4(NG_, T_, BF_) \
@@ -917,16 +942,17 @@ ICB_API int icb_paged_decode_q4(const void* record, void* stream) {
   Q4DecodeCall c;
   memcpy(&c, record, sizeof(c));
   if (c.rows <= 0) return 0;
-  if (c.hkv < 1 || c.hq < 1 || c.hq % c.hkv || c.tiles < 1 || c.plan == 0 || c.plan > (c.hd <= 128 ? 16 : 8) || c.q_stride % 8) return -2;
+  if (c.hkv < 1 || c.hq < 1 || c.hq % c.hkv || c.tiles < 1 || c.q_stride % 8) return -2;
+  if (c.plan == 0 || c.plan > (c.hd <= 128 ? 16 : 8)) return -2;
   const long long per = c.hq / c.hkv, slices = (per + 7) / 8, blocks = c.plan < 0 ? -c.plan : 0;
   // the numbers of a pool's tiles and of a row's tiles in all units are 32-bit
   if (c.max_blocks * c.tiles * c.hkv * slices > 0x7fffffffLL || c.max_blocks * c.tiles > 0x7ffffffLL ||
       c.num_blocks * c.hkv * c.tiles > 0x7fffffffLL || c.rows * c.hkv * slices > 0x7fffffffLL || c.hq > 0x7fffffffLL ||
       c.table_rows > 0x7fffffffLL || blocks > 0x7fffffffLL)
     return -2;
-  Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride, reinterpret_cast<int4*>(c.scratch), 0,
-                 c.scratch + (size_t)blocks * kQ4Warps * 4, (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8),
-                 (int)c.tiles, (int)c.max_blocks, (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
+  Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride,
+                 reinterpret_cast<int4*>(c.scratch), 0, c.scratch + (size_t)blocks * kQ4Warps * 4,
+                 (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8), (int)c.tiles, (int)c.max_blocks, (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
   return q4_variant<true>((int)c.hd, (int)per, (int)c.dtype, &a, (int)blocks, c.plan > 0 ? (int)c.plan : 0,
                           reinterpret_cast<cudaStream_t>(stream));
 }
