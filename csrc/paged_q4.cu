@@ -302,7 +302,7 @@ kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restr
   uint8_t* tile = pool + q4_tile_of(slot0, h0, hkv, tiles, 18 * HD);
   const uint16_t* from = keys ? k + (t0 + tok) * k_stride + h0 * HD + c * 8 : v + (t0 + tok) * v_stride + h0 * HD + r * 4;
 #pragma unroll 1
-  for (int h = h0; h < h1; ++h, tile += tiles * 18 * HD, from += HD) {
+  for (int h = h0; h < h1; ++h, tile += (size_t)tiles * 18 * HD, from += HD) {
     // rows that go one by one: bit i for row row0 + i, whose slot lane i has; pieces p0 to p1 of them
     long long row0 = first, slot = w.slot;
     uint32_t left = 0;
@@ -500,7 +500,7 @@ kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __rest
   const uint8_t* tile = pool + q4_tile_of(slot0, h0, hkv, tiles, 18 * HD);
   uint16_t* to = keys ? k + (t0 + tok) * pitch + h0 * HD + c * 8 : v + (t0 + tok) * pitch + h0 * HD + r * 4;
 #pragma unroll 1
-  for (int h = h0; h < h1; ++h, tile += tiles * 18 * HD, to += HD) {
+  for (int h = h0; h < h1; ++h, tile += (size_t)tiles * 18 * HD, to += HD) {
     if (w.leader >= 0) {
       const __half* scales = reinterpret_cast<const __half*>(tile + 16 * HD) + tok * 2 * NG;
       uint32_t word[NG];

@@ -132,7 +132,6 @@ struct Q4Query {
   uint32_t starts[NG > 4 ? 2 : 1];
   float start[T == 2 ? NG : 1][2];
   float factor[2];              // from the dot products to the base-2 score
-  uint32_t eight[NG];           // A fragments with -8 * 2^-24 in row g
 };
 
 template <int NG, int T, bool BF16>
@@ -157,8 +156,9 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* 
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 116);
-  const float up = __int_as_float((127 + 14 - e) << 23), up16 = up * 0.0625f;
-  const float back = __int_as_float((127 + 10 + e) << 23) * scale;           // 2^24 / up
+  const float up = copysignf(__int_as_float((127 + 14 - e) << 23), scale), up16 = up * 0.0625f;
+  // 2^24 / up * scale, which must send the -infinity of a masked score to itself: positive, the query having the sign of the scale
+  const float back = fmaxf(__int_as_float((127 + 10 + e) << 23) * fabsf(scale), 1.17549435e-38f);
   float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
@@ -190,8 +190,6 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* 
       f.starts[i] = *reinterpret_cast<const uint32_t*>(&both);
     }
   }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) f.eight[g] = r == g ? 0x80088008u : 0u;
 #pragma unroll
   for (int i = 0; i < 2; ++i) f.factor[i] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * i);
 }
@@ -244,8 +242,9 @@ struct Q4State {
 
 // T tiles of 16 tokens in shared memory, neighbours in the sequence. WHOLE: all of them belong to it; else `live` tokens do, bit
 // j of `gone`: tile T - 1 - j is not there. (Heads over 128 always go the second way: another copy of their code costs more than
-// the masks, 64 rows of 1000 tokens with heads of 256 take 16.6 us with it and 14.6 without.) With T = 2 both tiles go through the same columns' arithmetic at once: columns
-// 0 .. 3 are the heads over the first tile, 4 .. 7 over the second, which a group of at most four heads would leave idle.
+// the masks, 64 rows of 1000 tokens with heads of 256 take 16.6 us with it and 14.6 without.) With T = 2 both tiles go through
+// the same columns' arithmetic at once: columns 0 .. 3 are the heads over the first tile, 4 .. 7 over the second, which a group of
+// at most four heads would leave idle.
 template <int NG, int T, bool WHOLE>
 __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f, const uint8_t* tiles, int live,
                                         uint32_t gone) {
@@ -375,7 +374,8 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f
   for (int g = 0; g < NG; ++g) {
     const uint32_t b0 = transpose8(pack_f16x2(p[0] * sv[0][g], p[1] * sv[0][g]));
     const uint32_t b1 = transpose8(pack_f16x2(p[2] * sv[1][g], p[3] * sv[1][g]));
-    { const uint32_t eight = r == g ? 0x80088008u : 0u; mma_f16(st.z, eight, 0u, eight, 0u, b0, b1); }
+    const uint32_t eight = r == g ? 0x80088008u : 0u;                       // -8 * 2^-24 in row g
+    mma_f16(st.z, eight, 0u, eight, 0u, b0, b1);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const uint32_t mine = T == 1 ? 0xffffffffu : (r >> 2) == t ? 0xffffffffu : 0u;   // the columns of this tile
@@ -952,7 +952,8 @@ ICB_API int icb_paged_decode_q4(const void* record, void* stream) {
     return -2;
   Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride,
                  reinterpret_cast<int4*>(c.scratch), 0, c.scratch + (size_t)blocks * kQ4Warps * 4,
-                 (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8), (int)c.tiles, (int)c.max_blocks, (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
+                 (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8), (int)c.tiles, (int)c.max_blocks,
+                 (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
   return q4_variant<true>((int)c.hd, (int)per, (int)c.dtype, &a, (int)blocks, c.plan > 0 ? (int)c.plan : 0,
                           reinterpret_cast<cudaStream_t>(stream));
 }

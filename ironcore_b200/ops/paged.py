@@ -377,6 +377,8 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
         raise ValueError(f"query rows of {hq} heads of {hd} expected, got {tuple(shape)}")
     t, rows, per = shape[0], shape[:1], hq // hkv
     scale = hd ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= 1e38:
+        raise ValueError(f"a scale of {scale}")
     if block_table.dim() != 2 or block_table.dtype != i32 or seq_lens.dtype != i32 or seq_lens.shape != rows \
             or (seqs is not None and (seqs.dtype != i32 or seqs.shape != rows)):
         raise ValueError("block_table [S, pages], seq_lens [T] and seqs [T] must be int32")

@@ -135,6 +135,8 @@ class PagedCache:
         """:meth:`fork` for several sequences with one copy and one table update."""
         if copies < 0:
             raise ValueError("copies must not be negative")
+        if not set(seqs).isdisjoint(self._idle):
+            raise ValueError("only sequences from acquire() can be forked")
         partial = [self._host_lens[s] % self.block_size > 0 for s in seqs]
         if copies * len(seqs) > len(self._idle):
             raise RuntimeError("not enough idle cache sequences to fork")

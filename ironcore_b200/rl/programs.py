@@ -24,9 +24,10 @@ def _all_reduce(x, group):
 
 
 class TransformerProgram:
-    """The unified transformer on the block KV cache (``rl.kv_cache_bits``: 16 or 4). Prompts run the flash attention kernel on the packed projections
-    and scatter the rotated K / V rows into cache pages; all other rows append and attend over their pages. Tensor
-    parallelism uses the plain (non sequence-parallel) layout, one all-reduce after each row-parallel projection."""
+    """The unified transformer on the block KV cache (``rl.kv_cache_bits``: 16 or 4). Prompts run the flash attention
+    kernel on the packed projections and scatter the rotated K / V rows into cache pages; all other rows append and attend
+    over their pages. Tensor parallelism uses the plain (non sequence-parallel) layout, one all-reduce after each
+    row-parallel projection."""
 
     def __init__(self, model, config, max_seqs: int, max_seq_len: int, block_size: Optional[int],
                  num_blocks: Optional[int]):

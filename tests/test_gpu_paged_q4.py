@@ -112,7 +112,7 @@ def _check(q, pool, table, lens, hq, scale=None, **kw):
     from ironcore_b200.ops import paged
 
     hd, bs = pool.shape[3] // 18, 16 * pool.shape[2]
-    want, tol = O.attention(q.cpu(), *O.decoded(pool), table.cpu(), lens.cpu(), hq, scale or O.scale_of(hd),
+    want, tol = O.attention(q.cpu(), *O.decoded(pool), table.cpu(), lens.cpu(), hq, O.scale_of(hd) if scale is None else scale,
                             kw["seqs"].cpu() if "seqs" in kw else None)
     outs = []
     for t in (table, _widened(table, bs)):
@@ -175,6 +175,36 @@ def test_attention_with_queries_of_any_size(size):
     q = torch.randn((2, 4 * 128), generator=torch.Generator().manual_seed(1))
     q[0, 3:60] *= 2.0 ** -20                                # small elements beside large ones
     _check((q * size).to(BF).cuda(), pool, table, lens, 4, 0.09 / size)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-38])
+@pytest.mark.parametrize("hq", [2, 8])
+def test_attention_with_scales_of_any_sign(hq, scale):
+    """Tokens outside the sequence stay outside whatever the scores are multiplied with."""
+    pool, table, lens = O.cache([77, 300, 0, 1], 1, 128, 16, BF, seed=2, device="cuda")
+    _check(torch.randn((4, hq * 128), generator=torch.Generator().manual_seed(1)).to(BF).cuda(), pool, table, lens, hq, scale)
+
+
+def test_attention_in_place_and_over_nothing():
+    """The output over the query rows; no rows, tables without pages or rows, pools without pages."""
+    from ironcore_b200.ops import paged
+
+    pool, table, lens = O.cache([77, 3000, 0, 16], 2, 64, 16, BF, seed=2, device="cuda")
+    q = torch.randn((4, 6 * 64), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    for wide in (table, _widened(table, 16)):
+        want, over = paged.paged_decode_q4(q, pool, wide, lens, 6), q.clone()
+        assert paged.paged_decode_q4(over, pool, wide, lens, 6, out=over) is over and torch.equal(over, want)
+    assert paged.paged_decode_q4(q[:0], pool, table, lens[:0], 6).shape == (0, 6 * 64)
+    assert not paged.paged_decode_q4(q, pool, table[:, :0], lens, 6).any()
+    assert not paged.paged_decode_q4(q, pool[:0], table, lens, 6).any()
+    assert not paged.paged_decode_q4(q, pool, table[:0], lens, 6, seqs=torch.zeros(4, dtype=torch.int32, device="cuda")).any()
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    before = pool.clone()
+    paged.kv_append_q4(q[:0, :128], q[:0, 128:256], pool, none)
+    paged.kv_append_q4(q[:, :128], q[:, 128:256], pool[:0], torch.arange(4, device="cuda"))
+    assert torch.equal(pool, before)
+    assert paged.kv_read_q4(pool, none)[0].shape == (0, 128)
+    assert not paged.kv_read_q4(pool[:0], torch.arange(4, device="cuda"))[1].any()
 
 
 def test_attention_over_stale_pages():

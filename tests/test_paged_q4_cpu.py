@@ -115,7 +115,8 @@ def test_refusals():
     for a, kw in (((q, pool, table, lens, 3), {}), ((q, pool, table, lens, 2), {}), ((q, pool, table.long(), lens, 4), {}),
                   ((q, pool, table, lens.long(), 4), {}), ((q, pool, table, lens[:2], 4), {}), ((q, pool, table[:2], lens, 4), {}),
                   ((q, pool, table, lens, 4), {"seqs": lens.long()}), ((q, pool, table, lens, 4), {"out": torch.zeros((3, 128))}),
-                  ((q, pool, table, lens, 4), {"out": torch.zeros((3, 256)).half()}), ((q, pool, table, lens, 0), {})):
+                  ((q, pool, table, lens, 4), {"out": torch.zeros((3, 256)).half()}), ((q, pool, table, lens, 0), {}),
+                  ((q, pool, table, lens, 4, float("nan")), {}), ((q, pool, table, lens, 4, float("-inf")), {})):
         with pytest.raises(ValueError):
             paged.paged_decode_q4(*a, **kw)
 
@@ -196,6 +197,8 @@ def test_fork_is_all_or_nothing():
         c.fork(a, 2)                                        # pages
     with pytest.raises(ValueError):
         c.fork(a, -1)
+    with pytest.raises(ValueError):
+        c.fork(c._idle[0])                                  # nobody's sequence
     assert c.free_blocks == 1 and len(c._idle) == 2 and c.fork(a, 0) == []
     b, = c.fork(a)
     assert c.free_blocks == 0 and c.length(b) == 20
