@@ -25,9 +25,10 @@
 // Bounds. The bytes are 4.5 bits an element, each read once: at the copy bandwidth an SM gets a tile of 2304 bytes in about
 // 100 clocks, in which its four schedulers can issue 400 instructions; a tile takes about 300, of them 80 to unpack 4096 codes
 // and 21 matrix instructions (0.27 of their pipe). With 128 registers a thread, 16 warps on an SM issue 0.55 of the slots: the
-// kernels are held by the latencies of dependent instructions, not by memory. Measured in a row over inputs larger than L2: 512
-// rows of 768 tokens, 12 heads on 2 of 128: 31.5 us, 0.55 of the copy bandwidth; 4 rows of 100000, 32 on 8: 89 us, 0.79; 8 rows
-// of 4000, 32 on 32: 33 us, 0.68; 33 rows of 700, 12 on 12 of 64: 10.4 us.
+// kernels are held by the latencies of dependent instructions, not by memory. Captured calls over caches larger than L2, beside
+// the attention over the 16-bit cache: 512 rows of 768 tokens, 12 heads on 2 of 128, 29.8 us, 0.58 of the copy bandwidth (16 bits:
+// 109 us); 64 rows of 2000, 32 on 32, 107 us, 0.84 (391); 4 rows of 100000, 32 on 8, 87.5 us, 0.80 (382); 33 rows of up to 1500,
+// 12 on 12 of 64, 11.8 us (40); one row of 333, 5.7 us (9.8).
 #include <string.h>
 
 #include "host_common.h"
