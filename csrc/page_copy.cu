@@ -3,6 +3,7 @@
 //
 // Pairs are independent: no dst is another pair's src or dst. A pair with a page number outside the pool is left out.
 #include "host_common.h"
+#include "launch_behind.cuh"
 #include "ptx.cuh"
 
 namespace icb {
@@ -35,6 +36,7 @@ __host__ __device__ inline long long page_stretches(long long n) {
 
 template <typename VEC>
 __global__ void __launch_bounds__(kPageCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyArgs a) {
+  wait_for_previous();
   const uint32_t item = blockIdx.x;
   int p = 0;
   while (p + 1 < a.pools && item >= a.pool[p + 1].first_item) ++p;
@@ -67,8 +69,7 @@ static int launch_page_copy(PageCopyArgs& a, cudaStream_t st) {
   }
   if (items <= 0) return 0;
   if (items > 0x7fffffffLL) return -3;
-  page_copy_kernel<VEC><<<(unsigned)items, kPageCopyThreads, 0, st>>>(a);
-  return check_launch("page_copy");
+  return launch_behind("page_copy", page_copy_kernel<VEC>, (unsigned)items, kPageCopyThreads, 0, st, a);
 }
 
 }  // namespace icb

@@ -17,6 +17,7 @@
 #include <string.h>
 
 #include "host_common.h"
+#include "launch_behind.cuh"
 #include "ptx.cuh"
 #include "q4.cuh"
 
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(256)
 kv_append_q4_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint8_t* __restrict__ pool,
                     const long long* __restrict__ slots, long long total, int hkv, int hd, int tiles, long long num_slots,
                     long long k_stride, long long v_stride) {
+  wait_for_previous();
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const int per = hd / 4, piece = (int)(i % per);
   const long long th = i / per, t = th / hkv;
@@ -293,6 +295,7 @@ kv_append_q4_tile_kernel(const uint16_t* __restrict__ k, const uint16_t* __restr
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5, j = warp & 1;
   const int h0 = blockIdx.y * per, h1 = min(hkv, h0 + per);
   const long long first = (long long)blockIdx.x * 16;
+  wait_for_previous();
   const Q4Window w = q4_window(slots, first, T, num_slots);
   const uint32_t valid = __ballot_sync(0xffffffffu, lane < 16 && w.slot >= 0 && w.slot < num_slots);
   const uint32_t single = valid & ~w.covered & (0x1111u << warp);
@@ -473,6 +476,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(256)
 kv_read_q4_kernel(const uint8_t* __restrict__ pool, const long long* __restrict__ slots, uint16_t* __restrict__ k,
                   uint16_t* __restrict__ v, long long total, int hkv, int hd, int tiles, long long num_slots) {
+  wait_for_previous();
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= total) return;
   const int per = hd / 4, piece = (int)(i % per);
@@ -491,6 +495,7 @@ kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __rest
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5, j = warp & 1;
   const int h0 = blockIdx.y * per, h1 = min(hkv, h0 + per);
   const long long first = (long long)blockIdx.x * 16, pitch = (long long)hkv * HD;
+  wait_for_previous();
   const Q4Window w = q4_window(slots, first, T, num_slots);
   // this warp's share of the rows that fill no tile
   const uint32_t single = ~w.covered & (first + 16 <= T ? 0xffffu : (1u << (T - first)) - 1u) & (0x1111u << warp);
@@ -609,8 +614,8 @@ ICB_API int icb_kv_append_q4(const void* record, void* stream) {
     if ((c.rows + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) { \
       auto kernel = c.dtype == kBF16 ? kv_append_q4_tile_kernel<NG_, true> : kv_append_q4_tile_kernel<NG_, false>; \
-      kernel<<<grid, kQ4RowWarps * 32, 0, st>>>(c.k, c.v, c.pool, c.slots, c.rows, hkv, tiles, c.num_slots, c.k_stride, \
-                                                c.v_stride, per); \
+      return launch_behind("kv_append_q4", kernel, grid, kQ4RowWarps * 32, 0, st, c.k, c.v, c.pool, c.slots, c.rows, hkv, \
+                           tiles, c.num_slots, c.k_stride, c.v_stride, per); \
     }
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
@@ -618,10 +623,9 @@ ICB_API int icb_kv_append_q4(const void* record, void* stream) {
     const long long total = c.rows * hkv * (hd / 4), blocks = (total + 255) / 256;
     if (blocks > 0x7fffffffLL) return -3;
     auto kernel = c.dtype == kBF16 ? kv_append_q4_kernel<true> : kv_append_q4_kernel<false>;
-    kernel<<<(unsigned)blocks, 256, 0, st>>>(c.k, c.v, c.pool, c.slots, total, hkv, hd, tiles, c.num_slots, c.k_stride,
-                                             c.v_stride);
+    return launch_behind("kv_append_q4", kernel, (unsigned)blocks, 256, 0, st, c.k, c.v, c.pool, c.slots, total, hkv, hd, tiles,
+                         c.num_slots, c.k_stride, c.v_stride);
   }
-  return check_launch("kv_append_q4");
 }
 
 // Rows of the pool in 16 bits; zeros for a slot outside the pool.
@@ -638,7 +642,8 @@ ICB_API int icb_kv_read_q4(const void* record, void* stream) {
     if ((c.rows + 15) / 16 > 0x7fffffffLL || grid.y > 65535) return -3;
 #define ICB_RUN(NG_) { \
       auto kernel = c.dtype == kBF16 ? kv_read_q4_tile_kernel<NG_, true> : kv_read_q4_tile_kernel<NG_, false>; \
-      kernel<<<grid, kQ4RowWarps * 32, 0, st>>>(c.pool, c.slots, c.k, c.v, c.rows, hkv, tiles, c.num_slots, per); \
+      return launch_behind("kv_read_q4", kernel, grid, kQ4RowWarps * 32, 0, st, c.pool, c.slots, c.k, c.v, c.rows, hkv, tiles, \
+                           c.num_slots, per); \
     }
     ICB_Q4_SIZES(ICB_RUN)
 #undef ICB_RUN
@@ -646,7 +651,7 @@ ICB_API int icb_kv_read_q4(const void* record, void* stream) {
     const long long total = c.rows * hkv * (hd / 4), blocks = (total + 255) / 256;
     if (blocks > 0x7fffffffLL) return -3;
     auto kernel = c.dtype == kBF16 ? kv_read_q4_kernel<true> : kv_read_q4_kernel<false>;
-    kernel<<<(unsigned)blocks, 256, 0, st>>>(c.pool, c.slots, c.k, c.v, total, hkv, hd, tiles, c.num_slots);
+    return launch_behind("kv_read_q4", kernel, (unsigned)blocks, 256, 0, st, c.pool, c.slots, c.k, c.v, total, hkv, hd, tiles,
+                         c.num_slots);
   }
-  return check_launch("kv_read_q4");
 }

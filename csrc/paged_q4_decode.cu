@@ -5,8 +5,10 @@
 // Up to eight query heads of a kv head's group are the N dimension of mma.sync.m16n8k16 (fp16, fp32 sums), 16 tokens the M
 // dimension of K Q^T and 16 elements that of V^T P^T: every row of the matrix instructions is used.
 //   * A code needs no conversion: four bits at the bottom of an fp16 are the number n 2^-24, exact in the matrix
-//     instruction, so a word & 0x000f000f is two operands, & 0x00f000f0 two more that are 16 n 2^-24. The factor 16 is taken
-//     out of the query elements beforehand and out of the output rows at the end; shifted by 8 the word gives the other four.
+//     instruction, so a word & 0x000f000f is two operands, & 0x00f000f0 two more that are 16 n 2^-24; shifted by 8 the word gives
+//     the other four. The factor 16 is taken out of the query elements beforehand. Values are rows of the product, which may be
+//     any combinations of elements that can be solved for: n and n + 16 n', the lower and the upper bytes of the word as they
+//     are, which saves an instruction in five; n' is had from the two sums at the end, to 2^-18 of the row's magnitude.
 //   * q . (n - 8) = q . n - 8 sum q: the second part is a product of the key scales with a constant of the query, one matrix
 //     instruction for all groups (the constant as fp16 plus what fp16 leaves of it, 22 bits). On the value side another one,
 //     whose constant operand has -8 in row g, sums -8 p_t sv_tg from the same rounded products.
@@ -32,6 +34,7 @@
 #include <string.h>
 
 #include "host_common.h"
+#include "launch_behind.cuh"
 #include "ptx.cuh"
 #include "q4.cuh"
 
@@ -198,7 +201,8 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* 
 // Running state of a warp: this lane's part of eight columns.
 template <int NG>
 struct Q4State {
-  float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), columns 2c + (reg & 1); odd elements times 16
+  float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), columns 2c + (reg & 1); odd elements times
+                                // 16 and with the even one below added
   float z[4];                   // row g: -8 * sum of the rounded p * value scale of group g, in the units of o (even elements)
   float m[2], l[2];             // what is subtracted in columns 2c, 2c + 1 (equal in all lanes r), sum of this lane's p
   __device__ __forceinline__ void clear() {
@@ -381,9 +385,10 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f
     for (int t = 0; t < T; ++t) {
       const uint32_t mine = T == 1 ? 0xffffffffu : (r >> 2) == t ? 0xffffffffu : 0u;   // the columns of this tile
       const uint32_t x0 = b0 & mine, x1 = b1 & mine;
-      const uint32_t v0 = vw[t][g], v1 = vw[t][NG + g], w0 = v0 >> 8, w1 = v1 >> 8;
-      mma_f16(st.o[g][0], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, x0, x1);
-      mma_f16(st.o[g][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, x0, x1);
+      const uint32_t v0 = vw[t][g], v1 = vw[t][NG + g];
+      const uint32_t w0 = __byte_perm(v0, 0u, 0x4341u), w1 = __byte_perm(v1, 0u, 0x4341u);     // the upper bytes
+      mma_f16(st.o[g][0], v0 & 0x000f000fu, v0 & 0x00ff00ffu, v1 & 0x000f000fu, v1 & 0x00ff00ffu, x0, x1);
+      mma_f16(st.o[g][1], w0 & 0x000f000fu, w0, w1 & 0x000f000fu, w1, x0, x1);
     }
   }
 }
@@ -482,7 +487,8 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int plan_rows[kQ4Warps + 1];
   __shared__ long long plan_before[kQ4Warps + 1];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_previous();
+  let_next_begin();                              // the joining kernel
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hkv;
   const int worker = blockIdx.x * kQ4Warps + warp;
@@ -606,8 +612,8 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
-          const float4 o = make_float4((st.o[g][0][e] + z) * by, fmaf(st.o[g][0][2 + e], 0.0625f, z) * by,
-                                       (st.o[g][1][e] + z) * by, fmaf(st.o[g][1][2 + e], 0.0625f, z) * by);
+          const float4 o = make_float4((st.o[g][0][e] + z) * by, fmaf(st.o[g][0][2 + e] - st.o[g][0][e], 0.0625f, z) * by,
+                                       (st.o[g][1][e] + z) * by, fmaf(st.o[g][1][2 + e] - st.o[g][1][e], 0.0625f, z) * by);
           if (h >= heads || now.row >= a.rows) continue;
           uint16_t* to = a.out + (size_t)now.row * a.out_stride + (size_t)(head0 + h) * HD + 32 * g + 4 * r;
           if (whole) q4_store4<BF16>(to, o.x, o.y, o.z, o.w);
@@ -647,6 +653,7 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
   const int units = a.hkv * a.slices, row = blockIdx.x / units, unit = blockIdx.x - row * units, group = a.hq / a.hkv;
   const int kvh = a.slices == 1 ? unit : unit / a.slices, g0 = (unit - kvh * a.slices) * 8;
   const int heads = min(COLUMNS, group - g0), head0 = kvh * group + g0;
+  wait_for_previous();
   const int len = q4_len(a, row), n = q4_count(len), passes = (n + T - 1) / T;
   // passes warp, warp + warps, ... are this warp's; lane i looks up the place of its i-th tile from `listed` on
   uint8_t* ring = smem + warp * STAGES * STAGE;
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
     for (int g = 0; g < NG; ++g) {
       const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
       *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) =
-          make_float4(st.o[g][0][e] + z, fmaf(st.o[g][0][2 + e], 0.0625f, z), st.o[g][1][e] + z, fmaf(st.o[g][1][2 + e], 0.0625f, z));
+          make_float4(st.o[g][0][e] + z, fmaf(st.o[g][0][2 + e] - st.o[g][0][e], 0.0625f, z), st.o[g][1][e] + z, fmaf(st.o[g][1][2 + e] - st.o[g][1][e], 0.0625f, z));
     }
     if (r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
   }
@@ -753,8 +760,7 @@ paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long t
   __shared__ float sm_m[SETS], sm_l[SETS];
   const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4, group = a.hq / a.hkv;
   const long long task = SPREAD ? blockIdx.x : (long long)blockIdx.x * SETS + set;
-  // every block waits, also one without work: what follows this kernel follows the attention kernel too
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   if (task >= tasks || (!SPREAD && set >= SETS)) return;
   const long long entry = task / a.heads;
   const int h = (int)(task - entry * a.heads);
@@ -858,8 +864,7 @@ static int launch_q4_units(const Q4DecodeArgs& a, int warps, long long units, cu
       return -5;
     ready[dev] = 1;
   }
-  k<<<(unsigned)units, warps * 32, warps * each, st>>>(a);
-  return check_launch("paged_decode_q4");
+  return launch_behind("paged_decode_q4", k, (unsigned)units, warps * 32, warps * each, st, a);
 }
 
 template <int NG, int T, bool BF16>
@@ -867,24 +872,15 @@ static int launch_q4_decode(Q4DecodeArgs& a, int blocks, cudaStream_t st) {
   if (blocks > q4_blocks<NG, T, BF16>()) return -5;
   const long long units = (long long)a.rows * a.hkv * a.slices, workers = (long long)blocks * kQ4Warps;
   a.by_unit = units <= workers;                  // an entry for each unit or each warp, whichever are fewer
-  paged_decode_q4_kernel<NG, T, BF16><<<blocks, kQ4Threads, q4_smem<NG, T>(), st>>>(a);
-  // starts while the attention kernel runs out
+  const int rc = launch_behind("paged_decode_q4", paged_decode_q4_kernel<NG, T, BF16>, blocks, kQ4Threads, q4_smem<NG, T>(), st,
+                               a);
+  if (rc != 0) return rc;
   const bool spread = units * 8 < workers;       // more than eight parts to a unit
   const long long tasks = (a.by_unit ? units : workers) * a.heads;
   constexpr int SETS = kQ4MergeThreads / (NG * 8);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(spread ? tasks : (tasks + SETS - 1) / SETS));
-  cfg.blockDim = dim3(kQ4MergeThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = spread ? cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, true>, a, tasks)
-                               : cudaLaunchKernelEx(&cfg, paged_decode_q4_merge_kernel<NG, BF16, false>, a, tasks);
-  if (e != cudaSuccess) return -(int)e;
-  return check_launch("paged_decode_q4");
+  const unsigned grid = (unsigned)(spread ? tasks : (tasks + SETS - 1) / SETS);
+  auto merge = spread ? paged_decode_q4_merge_kernel<NG, BF16, true> : paged_decode_q4_merge_kernel<NG, BF16, false>;
+  return launch_behind("paged_decode_q4_merge", merge, grid, kQ4MergeThreads, 0, st, a, tasks);
 }
 
 // What a call needs of a variant: blocks of the kernel for ranges that fit the GPU (RUN false), or the call itself. T = 2 where

@@ -322,6 +322,65 @@ def test_attention_in_graphs():
     assert bool(((out.cpu().double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_calls_follow_one_another(wide):
+    """Every call reads what the one before wrote, with nothing in between: as with a synchronisation after each. Also from a
+    graph that forks to another stream and joins."""
+    from ironcore_b200.ops import paged
+
+    hkv, hd, hq, bs = 2, 128, 8, 16
+    first, table, lens = O.cache([40, 300, 5], hkv, hd, bs, BF, seed=3, device="cuda")
+    lens = lens - 1
+    table = _widened(table, bs) if wide else table
+    blocks = first.shape[0]
+    src, dst = (torch.tensor([b], dtype=torch.int32, device="cuda") for b in (int(table[1, 0]), blocks - 1))
+    index = torch.arange(3, device="cuda")
+    start = torch.randn((3, hq * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    side = torch.cuda.Stream()
+
+    def steps(pool, q, after, fork=False):
+        outs = []
+        for i in range(20):
+            slots = table[index, (lens // bs).long()].long() * bs + lens.long() % bs
+            paged.kv_append_q4(q[:, :hkv * hd], q[:, hkv * hd:2 * hkv * hd], pool, slots)
+            after()
+            out = paged.paged_decode_q4(q, pool, table, lens + 1, hq)
+            after()
+            if fork and i % 5 == 0:
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    extra = out.float().sum()
+            paged.copy_pages(pool[None], src, dst)
+            after()
+            k, v = paged.kv_read_q4(pool, torch.arange(bs, device="cuda") + (blocks - 1) * bs)
+            after()
+            if fork and i % 5 == 0:
+                torch.cuda.current_stream().wait_stream(side)
+            q = paged.paged_decode_q4(out, pool, table, lens + 1, hq, out=out)
+            after()
+            paged.kv_append_q4(k[:1], v[:1], pool, slots[:1])
+            after()
+            outs += [q, k, v]
+        return outs
+
+    pool = first.clone()
+    want = steps(pool, start, torch.cuda.synchronize)
+    again = first.clone()
+    for a, b in zip(steps(again, start, lambda: None), want):
+        assert torch.equal(a, b)
+    assert torch.equal(again, pool)
+    pool.copy_(first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = steps(again, start, lambda: None, fork=True)
+    for _ in range(3):
+        again.copy_(first)
+        graph.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_pools_larger_than_32_bit_offsets():
     """Pages on both sides of 2^31 and 2^32 bytes."""
     from ironcore_b200.ops import paged
