@@ -42,7 +42,9 @@ namespace icb {
 
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = kQ4Warps * 32;
-constexpr int kQ4MinTiles = 2;                  // least tiles of a warp
+// Least tiles of a warp: with fewer, joining the parts of a long row among short ones takes longer than what it gains. One row of
+// 8000 tokens among 255 of 100 (12 heads on 2): 42 us with 2, 23.5 with 6; 4 rows of 4000 (32 on 8): 14.6, 14.3, with 12 15.1.
+constexpr int kQ4MinTiles = 6;
 constexpr int kQ4Whole = 8;                     // units of at most so many tiles are not divided among warps
 constexpr float kQ4Top = 12.f;                  // log2 of the largest fp16 probability times scale right after a new maximum
 constexpr float kQ4Limit = 32768.f;             // and what it may grow to before the maximum is taken again: fp16 holds it
@@ -488,7 +490,6 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
   __shared__ int plan_rows[kQ4Warps + 1];
   __shared__ long long plan_before[kQ4Warps + 1];
   wait_for_previous();
-  let_next_begin();                              // the joining kernel
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hkv;
   const int worker = blockIdx.x * kQ4Warps + warp;
@@ -841,14 +842,19 @@ static int q4_blocks() {
 }
 
 // Warps of a block of the kernel for whole units; 0: the call goes to the kernel for ranges. Enough of them to fill the GPU with
-// ten warps to an SM, no more than two tiles each need. A warp with more than 32 tiles would hold the others up when the
-// lengths differ: 4 rows of 30000 tokens on 8 kv heads take 104 us here with 16 warps and 45 us in ranges, 512 rows of 768
-// tokens on 2 kv heads 37 us here with 2 warps and 43 us in ranges, 8 rows of 4000 on 32 kv heads 41 us here with 8 and 47 us.
+// ten warps to an SM, no more than two tiles each need, and so many that none has more than 32 tiles, for a long row among
+// short ones is its block's alone. Ranges cost some 10 us more, of which a part of a few tiles is too much to wait for them where
+// the units are few: what a warp has here beyond an even share of all tiles may be ten tiles of 128 elements a head. With
+// 128-element heads, this kernel and ranges, us: 512 rows of 768 tokens on 2 kv heads 28.8, 37.8; of 1536 46.8, 58.7; 8 of 4000 on
+// 32 30.4, 35.6; 64 of 8000 on 2 33.3, 43.7; 8 of 4000 on 8 16.8, 19.2; but 4 of 4000 on 8 16.3, 14.6; 16 of 8000 on 2 31.7, 20.5;
+// 4 of 30000 on 8 91, 35.7; 48 of up to 10000 on 8 39.7, 37.1. 64 rows of 4000 on 1 of 256: 36.8, 28.0.
 static int q4_unit_warps(int hd, long long units, long long tiles) {
   const int most = hd <= 128 ? 16 : 8;
   int warps = 1;
-  while (warps < most && units * warps < 10LL * num_sms() && tiles > 2 * warps) warps *= 2;
-  return tiles <= 32 * warps && units <= 0x7fffffffLL ? warps : 0;
+  while (warps < most && ((units * warps < 10LL * num_sms() && tiles > 2 * warps) || tiles > 32 * warps)) warps *= 2;
+  const long long held = (hd <= 64 ? 24LL : hd <= 128 ? 16LL : 8LL) * num_sms();       // warps that the GPU holds
+  const long long beyond = tiles / warps - units * tiles / held;
+  return tiles <= 32 * warps && beyond * hd <= 10 * 128 && units <= 0x7fffffffLL ? warps : 0;
 }
 
 template <int NG, int T, bool BF16>
