@@ -27,7 +27,7 @@ struct PageCopyArgs {
 };
 
 // A page is cut into the fewest equal stretches that a block moves with all its loads in flight. Equal: 4-bit pages of 18 KB and
-// the like would leave a short last stretch (448 pairs of 18 KB in 32 layers, from 64 pages: 58 us, now 51.5, 0.89 of the copy
+// the like would leave a short last stretch (448 pairs of 18 KB in 32 layers, from 64 pages: 58 us, now 50.3, 0.92 of the copy
 // bandwidth). Blocks that take neighbouring VECs across pages' borders need two divisions per access and wait for them (76 us).
 // 128 threads of 5 accesses: 8 KB pages, 448 pairs in 56 pools, 40.8 us; 256 of 4 45.5, 128 of 16 53.6.
 __host__ __device__ inline long long page_stretches(long long n) {

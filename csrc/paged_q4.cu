@@ -12,8 +12,8 @@
 // Two forms of each direction: one thread per 8 elements of a row, for few rows; and four warps per tile of 16 rows and head, in
 // the order of the tile's lanes, so that all 18 hd bytes of the tile leave or arrive in 512-byte pieces (a row by itself touches
 // all of a tile's value sectors, two bytes in each). Rows that do not fill a tile go one by one. 32768 rows of 8 heads of 128:
-// append 38 us, 0.69 of the copy bandwidth, held by instruction issue (0.7 of the slots: 6 instructions an element and the
-// groups' extremes); read 31 us, 0.84, held by its writes. One warp per tile took 61 and 39 us.
+// append 41 us, 0.64 of the copy bandwidth, held by instruction issue (0.68 of the slots: eleven instructions an element, half of
+// them conversion and rounding); read 32 us, 0.83, held by its writes. One warp per tile took 61 and 39 us.
 #include <string.h>
 
 #include "host_common.h"

@@ -25,12 +25,12 @@
 // line, cut evenly over the warps that the GPU holds, and a second kernel that joins the parts (Q4Plan).
 //
 // Bounds. The bytes are 4.5 bits an element, each read once: at the copy bandwidth an SM gets a tile of 2304 bytes in about
-// 100 clocks, in which its four schedulers can issue 400 instructions; a tile takes about 300, of them 80 to unpack 4096 codes
-// and 21 matrix instructions (0.27 of their pipe). With 128 registers a thread, 16 warps on an SM issue 0.55 of the slots: the
+// 100 clocks, in which its four schedulers can issue 400 instructions; a tile takes about 310, of them 72 to unpack 4096 codes
+// and 21 matrix instructions (0.28 of their pipe). With 128 registers a thread, 16 warps on an SM issue 0.57 of the slots: the
 // kernels are held by the latencies of dependent instructions, not by memory. Captured calls over caches larger than L2, beside
-// the attention over the 16-bit cache: 512 rows of 768 tokens, 12 heads on 2 of 128, 29.8 us, 0.58 of the copy bandwidth (16 bits:
-// 109 us); 64 rows of 2000, 32 on 32, 107 us, 0.84 (391); 4 rows of 100000, 32 on 8, 87.5 us, 0.80 (382); 33 rows of up to 1500,
-// 12 on 12 of 64, 11.8 us (40); one row of 333, 5.7 us (9.8).
+// the attention over the 16-bit cache: 512 rows of 768 tokens, 12 heads on 2 of 128, 28.8 us, 0.60 of the copy bandwidth (16 bits:
+// 109 us); 64 rows of 2000, 32 on 32, 100 us, 0.90 (388); 4 rows of 100000, 32 on 8, 84.8 us, 0.83 (385); 33 rows of up to 1500,
+// 12 on 12 of 64, 11.1 us (40); one row of 333, 5.2 us (9.6).
 #include <string.h>
 
 #include "host_common.h"
