@@ -152,6 +152,20 @@ def test_attention_over_long_contexts(hd, spread):
     _check(q, pool, table, lens, 6)
 
 
+@pytest.mark.parametrize("hd,group", [(128, 6), (128, 2), (64, 3), (256, 1)])
+def test_attention_of_blocks_over_long_rows(hd, group):
+    """A block's warps at their longest: 16 (8 for larger heads) with 32 tiles each, beside rows of all lengths."""
+    from ironcore_b200.ops import paged
+
+    longest = 8192 if hd <= 128 else 4096
+    lens = [longest, 1, 0, longest - 1, 17, 511, 513, longest // 2 + 5] + [16 * i + i % 3 for i in range(24)]
+    pool, table, lens = O.cache(lens, 4, hd, 16, BF, seed=4, device="cuda")
+    plan, _ = paged._q4_plan(hd, group, BF, 32 * 4, table.shape[1])
+    assert plan == (16 if hd <= 128 else 8)
+    _check(torch.randn((32, 4 * group * hd), generator=torch.Generator().manual_seed(1)).to(BF).cuda(), pool, table, lens,
+           4 * group)
+
+
 def test_attention_with_one_dominant_token():
     """A first token that takes nearly all probability and has tiny values, among values of ordinary size."""
     from ironcore_b200.ops import paged
