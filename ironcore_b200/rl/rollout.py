@@ -243,7 +243,7 @@ class RolloutEngine:
 
     def _generate_uniform(self, prompts, max_new_tokens, temperature, top_k, top_p, generator, samples):
         s, p = prompts.shape
-        prompts = prompts.to(self.device)
+        prompts = prompts.to(self.device, torch.int64)
         out = torch.empty((s * samples, p + max_new_tokens), dtype=torch.int64, device=self.device)
         out[:, :p] = prompts.repeat_interleave(samples, dim=0) if samples > 1 else prompts
         logps = torch.empty((s * samples, max_new_tokens), dtype=torch.float32, device=self.device)

@@ -362,3 +362,26 @@ def test_grpo_on_shared_prompts_and_four_bits(bits, share):
     st = tr.policy_update(batch)
     # the cache's rounding reaches the sampled tokens' log-probs, no more
     assert abs(st["ratio_mean"] - 1.0) < (1e-3 if bits == 16 else 0.2)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int16, torch.uint8, torch.float32])
+@pytest.mark.parametrize("family", ["llama", "tetepel"])
+def test_prompts_of_any_type(family, dtype):
+    """Token ids reach the model in 64 bits, which its kernels read, whatever the prompts' type."""
+    import tetepel_cases as T
+    from ironcore_b200.rl import RolloutEngine
+
+    if family == "llama":
+        c, model = _model()
+        eng, vocab = RolloutEngine(model, c, max_seqs=4, max_seq_len=64, block_size=16), 200
+    else:
+        cfg = T.config([T.layer(window=5)], streams=3, width=24)
+        model, c = T.build(cfg, T.weights(cfg))
+        eng, vocab = T.engine(model, c), min(200, cfg["vocab"])
+    prompts = torch.randint(0, vocab, (2, 9), generator=torch.Generator().manual_seed(4))
+    want, lp = eng.generate(prompts, 5, temperature=0.0)
+    seen, real = [], eng.program.logits
+    eng.program.logits = lambda batch: (seen.append(batch.tokens.dtype), real(batch))[1]
+    got, lp2 = eng.generate(prompts.to(dtype), 5, temperature=0.0)
+    assert set(seen) == {torch.int64}
+    assert torch.equal(got, want) and torch.equal(lp, lp2)
