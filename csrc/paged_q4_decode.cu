@@ -64,6 +64,7 @@ struct Q4DecodeArgs {
   int by_unit;                  // each unit of the call, or (by_unit 0) for each warp: the unit that begins in its range
   float* part;                  // [workers][2][slice heads] records of HD + 4 floats: outputs, maximum, sum
   int rows, hq, hkv, slices, heads, tiles, max_blocks, table_rows, num_blocks;   // heads: of a slice, at most eight
+  int workers;                  // warps that share the tiles
   float scale;                  // score factor times log2(e)
 };
 
@@ -406,7 +407,9 @@ __device__ __forceinline__ int q4_count(int len) { return (len + kQ4Tile - 1) / 
 // How the call's tiles are dealt out: unit = (row, slice of at most eight heads of a kv head), units in order, all tiles of all
 // units in one line that is cut into equal ranges, one for each warp, so that lengths of any mixture keep every warp busy for
 // the same time. A cut inside a unit of at most kQ4Whole tiles moves to its end: joining the parts of a short unit takes longer
-// than a few more tiles. Every block finds the places of its warps by a sum over the rows' lengths.
+// than a few more tiles. Every block finds the places of its warps by a sum over the rows' lengths. Lengths that change under
+// the call, which are read more than once, make its results worthless but lead nowhere: rows, units and workers are held within
+// their ranges here and where the parts are joined, and a cut within its unit.
 struct Q4Plan {
   long long total;              // tiles of the call
   long long per;                // of a warp
@@ -449,7 +452,7 @@ __device__ __forceinline__ Q4Plan q4_plan(const Q4DecodeArgs& a, int* rows, long
       if (at < (b + n) * plan.units) break;
       b += n;
     }
-    rows[w] = row;
+    rows[w] = min(row, a.rows - 1);
     before[w] = b * plan.units;
   }
   __syncthreads();
@@ -507,11 +510,11 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
       const int row = plan_rows[warp + i], len = q4_len(a, row), n = q4_count(len);
       const uint32_t into = (uint32_t)(at[i] - plan_before[warp + i]);
       const uint32_t unit = min(into / (uint32_t)max(n, 1), (uint32_t)plan.units - 1);
-      const uint32_t off = into - unit * n;
+      const int off = (int)min(into - unit * n, (uint32_t)n);
       now.row = row;
       now.unit = unit;
       now.len = len;
-      now.begin = -(int)off;
+      now.begin = -off;
       now.end = now.begin + n;
       if (off > 0 && n <= kQ4Whole) {
         at[i] += n - off;
@@ -543,7 +546,7 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
         entered = false;
       }
       const int kvh = a.slices == 1 ? ahead.unit : ahead.unit / a.slices;
-      const int row = min(ahead.row, a.rows - 1);          // lengths that change under the call must not lead out of bounds
+      const int row = min(ahead.row, a.rows - 1);
       if (!entered) {                                      // the unit's query rows travel with its first tile
         const int g0 = (ahead.unit - kvh * a.slices) * 8, pieces = min(COLUMNS, group - g0) * (HD / 8);
         const uint16_t* q = a.q + (size_t)row * a.q_stride + (size_t)(kvh * group + g0) * HD;
@@ -766,7 +769,10 @@ paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long t
   const long long entry = task / a.heads;
   const int h = (int)(task - entry * a.heads);
   const int4 owner = a.owner[entry];
-  if (owner.x < 0) return;
+  // -1: nothing to join; what else is out of range only lengths that changed under the call leave here
+  if ((uint32_t)owner.x >= (uint32_t)a.rows || (uint32_t)owner.y >= (uint32_t)(a.hkv * a.slices) || owner.z < 0 ||
+      owner.w >= a.workers)
+    return;
   const int kvh = owner.y / a.slices, g0 = (owner.y - kvh * a.slices) * 8;
   if (h >= group - g0) return;
   float top = kQ4None, sum = 0.f;
@@ -877,6 +883,7 @@ template <int NG, int T, bool BF16>
 static int launch_q4_decode(Q4DecodeArgs& a, int blocks, cudaStream_t st) {
   if (blocks > q4_blocks<NG, T, BF16>()) return -5;
   const long long units = (long long)a.rows * a.hkv * a.slices, workers = (long long)blocks * kQ4Warps;
+  a.workers = (int)workers;
   a.by_unit = units <= workers;                  // an entry for each unit or each warp, whichever are fewer
   const int rc = launch_behind("paged_decode_q4", paged_decode_q4_kernel<NG, T, BF16>, blocks, kQ4Threads, q4_smem<NG, T>(), st,
                                a);
@@ -956,7 +963,7 @@ ICB_API int icb_paged_decode_q4(const void* record, void* stream) {
   Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride,
                  reinterpret_cast<int4*>(c.scratch), 0, c.scratch + (size_t)blocks * kQ4Warps * 4,
                  (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8), (int)c.tiles, (int)c.max_blocks,
-                 (int)c.table_rows, (int)c.num_blocks, (float)c.scale * kLog2e};
+                 (int)c.table_rows, (int)c.num_blocks, 0, (float)c.scale * kLog2e};
   return q4_variant<true>((int)c.hd, (int)per, (int)c.dtype, &a, (int)blocks, c.plan > 0 ? (int)c.plan : 0,
                           reinterpret_cast<cudaStream_t>(stream));
 }

@@ -536,3 +536,33 @@ def test_rollouts(bits):
     assert t2.shape == t1.shape and torch.equal(t2[0], t2[1]) and torch.equal(t2[0], t2[2])
     again, lp3 = graph.generate(prompts, 24, temperature=0.0, samples=3)
     assert torch.equal(t2, again) and torch.equal(lp2, lp3)
+
+
+@pytest.mark.parametrize("rows,heads", [(5, 2), (500, 8)])
+def test_lengths_that_change_under_a_call(rows, heads):
+    """Another stream overwrites the lengths while calls over ranges of tiles run: what such calls give is worthless, but nothing
+    outside of their output is touched, and later calls are right. An entry for each unit, and one for each warp."""
+    from ironcore_b200.ops import paged
+
+    hd, bs = 64, 16
+    g = torch.Generator().manual_seed(rows)
+    most = 2000 if rows < 10 else 200
+    pool, table, lens = O.cache([most] * rows, heads, hd, bs, BF, seed=1, device="cuda")
+    table = _widened(table, bs)
+    q = torch.randn((rows, heads * 2 * hd), generator=g).to(BF).cuda()
+    plan, _ = paged._q4_plan(hd, 2, BF, rows * heads, table.shape[1])
+    assert plan < 0 and (rows * heads <= -4 * plan) == (rows < 10)
+    want = paged.paged_decode_q4(q, pool, table, lens, 2 * heads)
+    now = lens.clone()
+    others = [(torch.rand(rows, generator=g) ** 3 * (torch.rand(rows, generator=g) > 0.3) * most).int().cuda() for _ in range(20)]
+    guarded = torch.full((rows + 4, heads * 2 * hd), 7.0, dtype=BF, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for i in range(200):
+        with torch.cuda.stream(side):
+            for j in range(4):
+                now.copy_(others[(i + j) % 20] if j % 2 else lens)
+        paged.paged_decode_q4(q, pool, table, now, 2 * heads, out=guarded[2:-2])
+    torch.cuda.synchronize()
+    assert bool((guarded[:2] == 7).all()) and bool((guarded[-2:] == 7).all())
+    assert torch.equal(paged.paged_decode_q4(q, pool, table, lens, 2 * heads), want)
