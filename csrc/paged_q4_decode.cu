@@ -18,6 +18,7 @@
 //   * p_t sv_tg is rounded to fp16 too. Its range is held by the maximum that the softmax subtracts: it runs over
 //     log2 p_t + log2 max_g |sv_tg| instead of log2 p_t, so that the largest product is 2^12 to 2^15, whatever the values'
 //     magnitude. Relative error 2^-11 down to 2^-26 of the largest contribution; sums, maxima and p itself stay in fp32.
+//   * Scores may have any size: from 2^22 on a maximum in fp32 does not do, and dot products are compared instead (Q4State).
 // Tokens outside the sequence get probability and value scale zero by selection, so nothing stale in a page (NaN scales
 // included) reaches a result. A page number outside the pool counts as a page outside the sequence.
 //
@@ -31,6 +32,7 @@
 // the attention over the 16-bit cache: 512 rows of 768 tokens, 12 heads on 2 of 128, 28.8 us, 0.60 of the copy bandwidth (16 bits:
 // 109 us); 64 rows of 2000, 32 on 32, 100 us, 0.90 (388); 4 rows of 100000, 32 on 8, 84.8 us, 0.83 (385); 33 rows of up to 1500,
 // 12 on 12 of 64, 11.1 us (40); one row of 333, 5.2 us (9.6).
+#include <math.h>
 #include <string.h>
 
 #include "host_common.h"
@@ -48,7 +50,9 @@ constexpr int kQ4MinTiles = 6;
 constexpr int kQ4Whole = 8;                     // units of at most so many tiles are not divided among warps
 constexpr float kQ4Top = 12.f;                  // log2 of the largest fp16 probability times scale right after a new maximum
 constexpr float kQ4Limit = 32768.f;             // and what it may grow to before the maximum is taken again: fp16 holds it
-constexpr float kQ4None = -1e30f;               // maximum of no tokens
+constexpr float kQ4None = 3e38f, kQ4Far = 2e38f;            // Q4State::off of no tokens, and of scores from kQ4Large on
+constexpr float kQ4Large = 4194304.f;           // 2^22: up to here a maximum in fp32 is within 1/2 of itself
+constexpr int kQ4MostFactor = 99;               // log2 of the largest factor from dot products to scores (its mantissa apart)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Q4DecodeArgs {
@@ -62,10 +66,11 @@ struct Q4DecodeArgs {
   long long out_stride;
   int4* owner;                  // {row, unit, first, last worker} of a unit that several warps share, or row -1; one entry for
   int by_unit;                  // each unit of the call, or (by_unit 0) for each warp: the unit that begins in its range
-  float* part;                  // [workers][2][slice heads] records of HD + 4 floats: outputs, maximum, sum
+  float* part;                  // [workers][2][slice heads] records of HD + 4 floats: outputs, Q4State::end
   int rows, hq, hkv, slices, heads, tiles, max_blocks, table_rows, num_blocks;   // heads: of a slice, at most eight
   int workers;                  // warps that share the tiles
-  float scale;                  // score factor times log2(e)
+  float scale;                  // score factor times log2(e) without its power of two (0, or 0.7 to 1.5), the exponent of that
+  int scale_exp;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -142,7 +147,7 @@ struct Q4Query {
 };
 
 template <int NG, int T, bool BF16>
-__device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* q, int heads, float scale) {
+__device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* q, int heads, float scale, int scale_exp) {
   constexpr int HD = NG * 32;
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3, head = T == 1 ? r : r & 3;
   float x[NG][8];
@@ -162,10 +167,23 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* 
   }
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 116);
+  if (BF16 && __any_sync(0xffffffffu, top > 0.f && top < 5.4210109e-20f)) {     // below 2^-64: `up` alone may not reach
+    const bool lift = top < 5.4210109e-20f;
+    scale_exp -= lift ? 64 : 0;
+    top *= lift ? 18446744073709551616.f : 1.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[g][i] *= lift ? 18446744073709551616.f : 1.f;
+    }
+  }
+  const int e = min(max((__float_as_int(top) >> 23) - 127, -100), 127);
   const float up = copysignf(__int_as_float((127 + 14 - e) << 23), scale), up16 = up * 0.0625f;
-  // 2^24 / up * scale, which must send the -infinity of a masked score to itself: positive, the query having the sign of the scale
-  const float back = fmaxf(__int_as_float((127 + 10 + e) << 23) * fabsf(scale), 1.17549435e-38f);
+  // 2^24 / up * scale, which must send the -infinity of a masked score to itself: positive, the query having the sign of the scale.
+  // Dot products are multiples of 2^-72 (2^-24 each of the query, the code, the scale) below 2^18, so that beyond 2^99 a larger
+  // factor changes nothing: scores that differ at all do so by 2^27, and none is an infinity
+  const int back_exp = min(max(10 + e + scale_exp, -126), kQ4MostFactor);
+  const float back = fmaxf(__int_as_float((127 + back_exp) << 23) * fabsf(scale), 1.17549435e-38f);
   float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
@@ -201,13 +219,32 @@ __device__ __forceinline__ void q4_load_query(Q4Query<NG, T>& f, const uint8_t* 
   for (int i = 0; i < 2; ++i) f.factor[i] = __shfl_sync(0xffffffffu, back, 8 * c + 4 * i);
 }
 
-// Running state of a warp: this lane's part of eight columns.
+// Sums of several parts over tokens, each with its own {at, off} (Q4State): the one to bring them to is that of the largest
+// maximum (either of two that fp32 does not tell apart), and what a part is to be multiplied with.
+__device__ __forceinline__ float2 q4_larger(const float2& a, const float2& b, float factor) {
+  return fmaf(b.x, factor, -b.y) > fmaf(a.x, factor, -a.y) ? b : a;
+}
+__device__ __forceinline__ float q4_weight(const float2& part, const float2& all, float factor) {
+  return exp2_fast(fmaf(part.x - all.x, factor, all.y - part.y));
+}
+__device__ __forceinline__ float2 q4_from(const float2& x, int half) {         // of the lane with this bit 1
+  const int lane = (threadIdx.x & 29) | half;
+  return make_float2(__shfl_sync(0xffffffffu, x.x, lane), __shfl_sync(0xffffffffu, x.y, lane));
+}
+
+// Running state of a warp: this lane's part of eight columns. Of a dot product s, p = exp2((s - at) * factor + off). `at` is 0 as
+// long as the largest score is below kQ4Large. From there on a maximum rounded to fp32 would lie too far from the score it is
+// to be subtracted from (by 32 at 2^30: p of 2^32 or 2^-32), so `at` is the largest dot product, whose distance to others is
+// exact enough, and `off` stays small: both are in shared memory, and kQ4Far for an `off` sends every pass there. That such
+// scores may come costs others little (512 rows of 768 tokens 29.0 -> 29.2 us, 78 of 264 11.9 -> 12.5); the difference to `at` in
+// every pass instead took 30.3 us.
 template <int NG>
 struct Q4State {
   float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), columns 2c + (reg & 1); odd elements times
                                 // 16 and with the even one below added
   float z[4];                   // row g: -8 * sum of the rounded p * value scale of group g, in the units of o (even elements)
-  float m[2], l[2];             // what is subtracted in columns 2c, 2c + 1 (equal in all lanes r), sum of this lane's p
+  float off[2], l[2];           // of columns 2c, 2c + 1 (equal in all lanes r); sum of this lane's p
+  float2* far;                  // this lane's {at, off} of both where `off` is kQ4Far
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -215,9 +252,10 @@ struct Q4State {
       for (int i = 0; i < 4; ++i) o[g][0][i] = o[g][1][i] = 0.f;
     }
     z[0] = z[1] = z[2] = z[3] = 0.f;
-    m[0] = m[1] = kQ4None;
+    off[0] = off[1] = kQ4None;
     l[0] = l[1] = 0.f;
   }
+  __device__ __forceinline__ float2 place(int e) const { return off[e] == kQ4Far ? far[e] : make_float2(0.f, off[e]); }
   __device__ __forceinline__ void rescale(int e, float by) {
     l[e] *= by;
     z[e] *= by;
@@ -227,13 +265,30 @@ struct Q4State {
       for (int t = 0; t < 2; ++t) { o[g][t][e] *= by; o[g][t][2 + e] *= by; }
     }
   }
+  // The end of a part's record: {off, sum}, or {kQ4Far, sum, at, factor} with all sums of the column as for an `off` of 0.
+  __device__ __forceinline__ float4 end(int e, float factor) {
+    float at = 0.f;
+    if (off[e] == kQ4Far) {
+      at = far[e].x;
+      rescale(e, exp2_fast(-far[e].y));
+    }
+    return make_float4(off[e], l[e], at, factor);
+  }
   // Columns n and n + 4 hold the same head over different tokens: both become their sum.
-  __device__ __forceinline__ void fold() {
+  __device__ __forceinline__ void fold(const float (&factor)[2]) {
+    const bool large = __any_sync(0xffffffffu, off[0] == kQ4Far || off[1] == kQ4Far);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float other = __shfl_xor_sync(0xffffffffu, m[e], 2), next = fmaxf(m[e], other);
-      rescale(e, exp2_fast(m[e] - next));
-      m[e] = next;
+      if (large) {
+        const float2 mine = place(e), both = q4_larger(q4_from(mine, 0), q4_from(mine, 2), factor[e]);
+        rescale(e, q4_weight(mine, both, factor[e]));
+        off[e] = both.x != 0.f ? kQ4Far : both.y;
+        far[e] = both;
+      } else {
+        const float next = fminf(off[e], __shfl_xor_sync(0xffffffffu, off[e], 2));
+        rescale(e, exp2_fast(next - off[e]));
+        off[e] = next;
+      }
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       z[e] += __shfl_xor_sync(0xffffffffu, z[e], 2);
 #pragma unroll
@@ -349,21 +404,50 @@ __device__ __forceinline__ void q4_pass(Q4State<NG>& st, const Q4Query<NG, T>& f
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    p[i] = exp2_fast(fmaf(s[i], f.factor[i & 1], -st.m[i & 1]));
+    p[i] = exp2_fast(fmaf(s[i], f.factor[i & 1], st.off[i & 1]));
     top = fmaxf(top, p[i] * reach[i >> 1]);
   }
   if (__any_sync(0xffffffffu, top > kQ4Limit)) {
+    float next[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float most = fmaxf(fmaf(s[e], f.factor[e], log2_fast(reach[0])), fmaf(s[2 + e], f.factor[e], log2_fast(reach[1])));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-      const float next = fmaxf(st.m[e], most - kQ4Top);
-      st.rescale(e, exp2_fast(st.m[e] - next));
-      st.m[e] = next;
-      p[e] = exp2_fast(fmaf(s[e], f.factor[e], -next));
-      p[2 + e] = exp2_fast(fmaf(s[2 + e], f.factor[e], -next));
+      next[e] = fminf(st.off[e], kQ4Top - most);
+    }
+    const bool far[2] = {fabsf(next[0]) >= kQ4Large, fabsf(next[1]) >= kQ4Large};       // also a column without a token yet
+    if (__any_sync(0xffffffffu, far[0] || far[1] || st.off[0] == kQ4Far || st.off[1] == kQ4Far)) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 old = st.place(e);
+        float dot = fmaxf(s[e], s[2 + e]);
+        dot = fmaxf(dot, __shfl_xor_sync(0xffffffffu, dot, 4));
+        dot = fmaxf(dot, __shfl_xor_sync(0xffffffffu, dot, 8));
+        dot = fmaxf(dot, __shfl_xor_sync(0xffffffffu, dot, 16));
+        float2 now = make_float2(old.x != 0.f ? fmaxf(old.x, dot) : far[e] && dot > -INFINITY ? dot : 0.f, 0.f);
+        float most = fmaxf(fmaf(s[e] - now.x, f.factor[e], log2_fast(reach[0])),
+                           fmaf(s[2 + e] - now.x, f.factor[e], log2_fast(reach[1])));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+        const float same = fmaf(now.x - old.x, f.factor[e], old.y);           // what would leave every p as it is
+        now.y = fminf(same, kQ4Top - most);
+        st.rescale(e, exp2_fast(now.y - same));
+        st.far[e] = now;
+        st.off[e] = now.x != 0.f ? kQ4Far : now.y;
+        p[e] = exp2_fast(fmaf(s[e] - now.x, f.factor[e], now.y));
+        p[2 + e] = exp2_fast(fmaf(s[2 + e] - now.x, f.factor[e], now.y));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        st.rescale(e, exp2_fast(next[e] - st.off[e]));
+        st.off[e] = next[e];
+        p[e] = exp2_fast(fmaf(s[e], f.factor[e], next[e]));
+        p[2 + e] = exp2_fast(fmaf(s[2 + e], f.factor[e], next[e]));
+      }
     }
   }
 #pragma unroll
@@ -459,6 +543,28 @@ __device__ __forceinline__ Q4Plan q4_plan(const Q4DecodeArgs& a, int* rows, long
   return plan;
 }
 
+// Four outputs of a head, at d, and its sum, of parts some of which have large scores: record(i) is the i-th one's.
+template <typename R>
+__device__ __forceinline__ void q4_join_large(float& sum, float4& acc, int parts, int d, R record, int hd) {
+  float2 all = make_float2(0.f, kQ4None);
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i = 0; i < 2 * parts; ++i) {
+    const float* x = record(i < parts ? i : i - parts);
+    const float4 end = *reinterpret_cast<const float4*>(x + hd);
+    const float2 place = end.x == kQ4Far ? make_float2(end.z, 0.f) : make_float2(0.f, end.x);
+    if (i < parts) {
+      all = q4_larger(all, place, end.w);
+      continue;
+    }
+    const float4 o = *reinterpret_cast<const float4*>(x + d);
+    const float by = q4_weight(place, all, end.w);
+    sum += end.y * by;
+    acc.x += o.x * by; acc.y += o.y * by; acc.z += o.z * by; acc.w += o.w * by;
+  }
+}
+
 // A place in the line of tiles, relative to the warp's first.
 struct Q4Cursor {
   int row, unit;                // unit within the row
@@ -492,6 +598,7 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int plan_rows[kQ4Warps + 1];
   __shared__ long long plan_before[kQ4Warps + 1];
+  __shared__ float2 far[kQ4Threads][2];
   wait_for_previous();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int group = a.hq / a.hkv;
@@ -580,6 +687,7 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
 
     Q4Query<NG, T> f;
     Q4State<NG> st;
+    st.far = far[threadIdx.x];
     int mine = 0;
     const uint8_t* tiles = ring;
     for (;;) {
@@ -592,7 +700,7 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();                            // all lanes' pieces have landed; the previous stage has been read
         const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
-        if (first) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
+        if (first) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale, a.scale_exp);
         issue();
         if (NG <= 4 && live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
         else q4_pass<NG, T, false>(st, f, tiles, live, gone);
@@ -606,12 +714,13 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], off);
       }
-      if (T == 2) st.fold();
+      if (T == 2) st.fold(f.factor);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = 2 * c + e;
         // slot 0: the unit began before this range; slot 1: it goes on after it
         float* rec = a.part + (((size_t)worker * 2 + (begins ? 1 : 0)) * a.heads + h) * REC;
+        const float4 end = st.end(e, f.factor[e]);
         const float by = !whole ? 16777216.f : st.l[e] == 0.f ? 0.f : 16777216.f / st.l[e];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -623,7 +732,7 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
           if (whole) q4_store4<BF16>(to, o.x, o.y, o.z, o.w);
           else *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) = o;
         }
-        if (!whole && h < heads && r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
+        if (!whole && h < heads && r == 0) *reinterpret_cast<float4*>(rec + HD) = end;
       }
       if (begins) {
         owner = whole ? make_int4(-1, 0, 0, 0) : make_int4(now.row, now.unit, worker, (int)((start + now.end - 1) / plan.per));
@@ -644,6 +753,13 @@ paged_decode_q4_kernel(const __grid_constant__ Q4DecodeArgs a) {
       for (int u = threadIdx.x; u < plan.units; u += kQ4Threads) a.owner[(size_t)row * plan.units + u] = make_int4(-1, 0, 0, 0);
   }
 }
+
+// Shared memory of one of its warps, besides Q4State::far: the ring, and once that is done with, a record of each column.
+template <int NG, int T> __host__ __device__ constexpr int q4_each() {
+  constexpr int ring = q4_stages<NG, T>() * q4_stage<NG, T>(), records = 8 * (NG * 32 + 4) * 4;
+  return ring > records ? ring : records;
+}
+constexpr int kQ4FarBytes = 32 * 2 * sizeof(float2);
 
 // A block for each unit, whose warps take turns with its tiles and meet in shared memory: one launch, nothing to plan, two
 // dependent loads before the first tile. For tables so narrow that the longest unit keeps its warps busy only shortly.
@@ -696,13 +812,14 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
   }
   Q4Query<NG, T> f;
   Q4State<NG> st;
+  st.far = reinterpret_cast<float2*>(smem + warps * q4_each<NG, T>()) + 2 * threadIdx.x;
   st.clear();
   const uint8_t* tiles = ring;
   for (int pass = warp; pass < passes; pass += warps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                // all lanes' pieces have landed; the previous stage has been read
     const uint32_t gone = missing >> ((STAGES - 2) * T) & ((1u << T) - 1u);
-    if (pass == warp) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale);
+    if (pass == warp) q4_load_query<NG, T, BF16>(f, tiles + T * TILE, heads, a.scale, a.scale_exp);
     issue();
     const int live = len - pass * T * kQ4Tile;
     if (NG <= 4 && live >= T * kQ4Tile && gone == 0u) q4_pass<NG, T, true>(st, f, tiles, live, gone);
@@ -720,30 +837,39 @@ __global__ void __launch_bounds__(NG <= 4 ? 512 : 256) paged_decode_q4_unit_kern
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     float* rec = records + (warp * 8 + 2 * c + e) * REC;
+    const float4 end = st.end(e, f.factor[e]);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const float z = __shfl_sync(0xffffffffu, st.z[e], 4 * g + c);
       *reinterpret_cast<float4*>(rec + 32 * g + 4 * r) =
           make_float4(st.o[g][0][e] + z, fmaf(st.o[g][0][2 + e] - st.o[g][0][e], 0.0625f, z), st.o[g][1][e] + z, fmaf(st.o[g][1][2 + e] - st.o[g][1][e], 0.0625f, z));
     }
-    if (r == 0) *reinterpret_cast<float2*>(rec + HD) = make_float2(st.m[e], st.l[e]);
+    if (r == 0) *reinterpret_cast<float4*>(rec + HD) = end;
   }
   __syncthreads();
   const int parts = min(warps, passes) * T;      // of a head: column h of each warp, and h + 4 with T = 2
   for (int i = threadIdx.x; i < heads * (HD / 4); i += blockDim.x) {
     const int h = i / (HD / 4), d = (i - h * (HD / 4)) * 4;
     const float* rec = records + h * REC;
-    float top = kQ4None, sum = 0.f;
+    float off = kQ4None, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, rec[p * COLUMNS * REC + HD]);
+    bool large = false;
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) {
-      const float* x = rec + p * COLUMNS * REC;
-      const float by = exp2_fast(x[HD] - top);
-      const float4 o = *reinterpret_cast<const float4*>(x + d);
-      sum += x[HD + 1] * by;
-      acc.x += o.x * by; acc.y += o.y * by; acc.z += o.z * by; acc.w += o.w * by;
+      off = fminf(off, rec[p * COLUMNS * REC + HD]);
+      large |= rec[p * COLUMNS * REC + HD] == kQ4Far;
+    }
+    if (large) {
+      q4_join_large(sum, acc, parts, d, [&](int p) { return rec + p * COLUMNS * REC; }, HD);
+    } else {
+#pragma unroll 4
+      for (int p = 0; p < parts; ++p) {
+        const float* x = rec + p * COLUMNS * REC;
+        const float by = exp2_fast(off - x[HD]);
+        const float4 o = *reinterpret_cast<const float4*>(x + d);
+        sum += x[HD + 1] * by;
+        acc.x += o.x * by; acc.y += o.y * by; acc.z += o.z * by; acc.w += o.w * by;
+      }
     }
     const float by = sum == 0.f ? 0.f : 16777216.f / sum;
     uint16_t* to = a.out + (size_t)row * a.out_stride + (size_t)(head0 + h) * HD + d;
@@ -761,7 +887,7 @@ __global__ void __launch_bounds__(kQ4MergeThreads)
 paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long tasks) {
   constexpr int HD = NG * 32, REC = HD + 4, LANES = HD / 4, SETS = kQ4MergeThreads / LANES, DEPTH = 8;
   __shared__ __align__(16) float sm_o[SPREAD ? SETS : 1][HD];
-  __shared__ float sm_m[SETS], sm_l[SETS];
+  __shared__ float sm_off[SETS], sm_l[SETS];
   const int set = threadIdx.x / LANES, d = (threadIdx.x - set * LANES) * 4, group = a.hq / a.hkv;
   const long long task = SPREAD ? blockIdx.x : (long long)blockIdx.x * SETS + set;
   wait_for_previous();
@@ -775,55 +901,61 @@ paged_decode_q4_merge_kernel(const __grid_constant__ Q4DecodeArgs a, long long t
     return;
   const int kvh = owner.y / a.slices, g0 = (owner.y - kvh * a.slices) * 8;
   if (h >= group - g0) return;
-  float top = kQ4None, sum = 0.f;
+  float off = kQ4None, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool large = false;
   constexpr int STEP = SPREAD ? SETS : 1;
+  auto record = [&](int w) { return a.part + (((size_t)w * 2 + (w == owner.z ? 1 : 0)) * a.heads + h) * REC; };
   for (int w0 = owner.z + (SPREAD ? set : 0); w0 <= owner.w && set < SETS; w0 += DEPTH * STEP) {
-    float2 ml[DEPTH];
+    float2 x[DEPTH];
     float4 o[DEPTH];
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {            // all on the way before the first is used
       const int w = w0 + i * STEP;
-      ml[i] = make_float2(kQ4None, 0.f);
+      x[i] = make_float2(kQ4None, 0.f);
       o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (w > owner.w) continue;
-      const float* rec = a.part + (((size_t)w * 2 + (w == owner.z ? 1 : 0)) * a.heads + h) * REC;
-      ml[i] = *reinterpret_cast<const float2*>(rec + HD);
+      const float* rec = record(w);
+      x[i] = *reinterpret_cast<const float2*>(rec + HD);
       o[i] = *reinterpret_cast<const float4*>(rec + d);
     }
-    float next = top;
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) next = fmaxf(next, ml[i].x);
-    const float x = exp2_fast(top - next);
-    sum *= x; acc.x *= x; acc.y *= x; acc.z *= x; acc.w *= x;
+    float next = off;
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {
-      const float y = exp2_fast(ml[i].x - next);
-      sum += ml[i].y * y;
+      next = fminf(next, x[i].x);
+      large |= x[i].x == kQ4Far;
+    }
+    const float by = exp2_fast(next - off);
+    sum *= by; acc.x *= by; acc.y *= by; acc.z *= by; acc.w *= by;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const float y = exp2_fast(next - x[i].x);
+      sum += x[i].y * y;
       acc.x += o[i].x * y; acc.y += o[i].y * y; acc.z += o[i].z * y; acc.w += o[i].w * y;
     }
-    top = next;
+    off = next;
   }
   if (SPREAD) {
     if (set < SETS) {
       *reinterpret_cast<float4*>(&sm_o[set][d]) = acc;
-      if (d == 0) { sm_m[set] = top; sm_l[set] = sum; }
+      if (d == 0) { sm_off[set] = off; sm_l[set] = sum; }
     }
-    __syncthreads();
+    large = __syncthreads_or(large);
     if (set > 0) return;
     float all = kQ4None;
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) all = fmaxf(all, sm_m[s]);
+    for (int s = 0; s < SETS; ++s) all = fminf(all, sm_off[s]);
     sum = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
-      const float x = exp2_fast(sm_m[s] - all);
+      const float x = exp2_fast(all - sm_off[s]);
       const float4 v = *reinterpret_cast<const float4*>(&sm_o[s][d]);
       sum += sm_l[s] * x;
       acc.x += v.x * x; acc.y += v.y * x; acc.z += v.z * x; acc.w += v.w * x;
     }
   }
+  if (large) q4_join_large(sum, acc, owner.w - owner.z + 1, d, [&](int i) { return record(owner.z + i); }, HD);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   q4_store4<BF16>(a.out + (size_t)owner.x * a.out_stride + (size_t)(kvh * group + g0 + h) * HD + d, acc.x * inv, acc.y * inv,
                   acc.z * inv, acc.w * inv);
@@ -866,8 +998,7 @@ static int q4_unit_warps(int hd, long long units, long long tiles) {
 template <int NG, int T, bool BF16>
 static int launch_q4_units(const Q4DecodeArgs& a, int warps, long long units, cudaStream_t st) {
   auto k = paged_decode_q4_unit_kernel<NG, T, BF16>;
-  constexpr int ring = q4_stages<NG, T>() * q4_stage<NG, T>(), record = 8 * (NG * 32 + 4) * 4;
-  constexpr int each = ring > record ? ring : record;
+  constexpr int each = q4_each<NG, T>() + kQ4FarBytes;
   static int ready[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -963,7 +1094,8 @@ ICB_API int icb_paged_decode_q4(const void* record, void* stream) {
   Q4DecodeArgs a{c.q, c.q_stride, c.pool, c.block_table, c.seqs, c.lens, c.out, c.out_stride,
                  reinterpret_cast<int4*>(c.scratch), 0, c.scratch + (size_t)blocks * kQ4Warps * 4,
                  (int)c.rows, (int)c.hq, (int)c.hkv, (int)slices, (int)(per < 8 ? per : 8), (int)c.tiles, (int)c.max_blocks,
-                 (int)c.table_rows, (int)c.num_blocks, 0, (float)c.scale * kLog2e};
+                 (int)c.table_rows, (int)c.num_blocks, 0, 0.f, 0};
+  a.scale = (float)frexp(c.scale, &a.scale_exp) * kLog2e;
   return q4_variant<true>((int)c.hd, (int)per, (int)c.dtype, &a, (int)blocks, c.plan > 0 ? (int)c.plan : 0,
                           reinterpret_cast<cudaStream_t>(stream));
 }

@@ -368,7 +368,7 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
     """q [T, hq * hd] (row view, any pitch): row i against the first ``seq_lens[i]`` tokens of the sequence whose pages are
     row ``seqs[i]`` of ``block_table`` (int32; None: row i) -> [T, hq * hd], into ``out`` (rows of any pitch) if given.
     A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens. A NaN
-    among the keys or values of a sequence makes the heads that read it NaN."""
+    among the keys or values of a sequence makes the heads that read it NaN. ``scale``: up to 1e38 of either sign."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
     shape, dtype, i32 = q.shape, q.dtype, torch.int32
     if hq < 1 or hq % hkv:

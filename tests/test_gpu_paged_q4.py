@@ -566,3 +566,92 @@ def test_lengths_that_change_under_a_call(rows, heads):
     torch.cuda.synchronize()
     assert bool((guarded[:2] == 7).all()) and bool((guarded[-2:] == 7).all())
     assert torch.equal(paged.paged_decode_q4(q, pool, table, lens, 2 * heads), want)
+
+
+@pytest.mark.parametrize("hq", [2, 8])
+@pytest.mark.parametrize("scale", [1.0, 16.0, -64.0, 2.0 ** 12, 2.0 ** 30, -2.0 ** 30, 1e31, -1e31, 1e36, 1e38, -1e38])
+@pytest.mark.parametrize("base", [-(2.0 ** 20), 2.0 ** 20, -3.0])
+def test_attention_with_scores_of_any_size(hq, scale, base):
+    """Scores ``scale`` * (``base`` + k / 8), k in -8 .. 7, whose dot products fp32 holds exactly: the softmax is that of the
+    differences, equal ones share, and scores that are all very negative are no empty row. Tolerance: a weight is off by 2^-21 of
+    1 + its distance in base 2 from the largest (the factor, its product with the difference and exp2, 2^-23 each); the product
+    with the value's scale by 2^-11, times codes of up to 15; the output by half a step of bf16."""
+    from ironcore_b200.ops import paged
+
+    hd, n = 128, 700
+    g = torch.Generator().manual_seed(5)
+    k, v = torch.zeros((n + 4, hd)), torch.randn((n + 4, hd), generator=g)
+    k[:, 0] = -4.0 if base > -4 and base < 0 else 4.0
+    k[:, 32] = -1.0                                         # the scale of the second group, whatever the element that counts
+    k[:, 40] = torch.randint(-8, 8, (n + 4,), generator=g) / 8.0
+    q = torch.zeros((2, hq, hd))
+    q[..., 0] = base / float(k[0, 0])
+    q[..., 40] = 1.0
+    q = q.view(2, hq * hd).to(BF)
+    pool = torch.zeros(paged.q4_pool_shape(44, 1, 16, hd), dtype=torch.uint8)
+    paged.kv_append_q4_reference(k.to(BF), v.to(BF), pool, torch.arange(n + 4))
+    kk, vv = (x.flatten(0, 1)[:, 0] for x in O.decoded(pool))
+    assert torch.equal(kk[:n + 4], k.double())
+    table = torch.arange(44, dtype=torch.int32)[None].repeat(2, 1).cuda()
+    lens = torch.tensor([n, 5], dtype=torch.int32).cuda()
+    for t in (table, _widened(table, 16)):
+        out = paged.paged_decode_q4(q.cuda(), pool.cuda(), t, lens, hq, scale).cpu().double().view(2, hq, hd)
+        for row, m in enumerate((n, 5)):
+            s = (kk[:m] @ q[row, :hd].double()) * scale
+            p = torch.softmax(s, 0)
+            off = 2.0 ** -21 * (1 + (s.max() - s).clamp(max=1e6) / 0.693)
+            step = vv[:m].abs().unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(-2) / 7
+            want = p @ vv[:m]
+            tol = 1.1 * (2.0 ** -11 * 15 * (p @ step) + 2 * ((p * off) @ vv[:m].abs()) + 2.0 ** -8 * want.abs()) + 1e-30
+            assert bool(((out[row] - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("hq", [2, 8])
+@pytest.mark.parametrize("big", [2.0 ** 18, -(2.0 ** 18)])
+def test_attention_with_scores_of_all_sizes(hq, big):
+    """Scores around ``big`` * {-4, 0, 3} * 64 in one row, the largest first, last or in between: between them only the largest
+    count, in either kernel's order and where parts of a row are joined. Tolerance as above."""
+    from ironcore_b200.ops import paged
+
+    hd, n, scale = 128, 1500, 64.0
+    g = torch.Generator().manual_seed(6)
+    pools, rows = [], []
+    for part in ((0, 400), (700, 720), (1100, n), (0, n), (n, n)):
+        k, v = torch.zeros((n + 4, hd)), torch.randn((n + 4, hd), generator=g)
+        low = torch.arange(n + 4) % 3 == 0                  # some very small ones everywhere
+        k[:, 0] = torch.where(low, 3.0 if big < 0 else -4.0, 0.0)
+        k[part[0]:part[1], 0] = torch.where(torch.rand(part[1] - part[0], generator=g) < 0.5, -4.0 if big < 0 else 3.0, 0.0)
+        k[:, 1] = torch.where(torch.arange(n + 4) % 2 == 0, -4.0, 3.5)      # the scale of the first group, whatever counts
+        k[:, 32] = -1.0
+        k[:, 40] = torch.randint(-8, 8, (n + 4,), generator=g) / 8.0
+        pools.append((k, v))
+    pool = torch.zeros(paged.q4_pool_shape(94 * 5, 1, 16, hd), dtype=torch.uint8)
+    for i, (k, v) in enumerate(pools):
+        paged.kv_append_q4_reference(k.to(BF), v.to(BF), pool, torch.arange(n + 4) + 94 * 16 * i)
+    q = torch.zeros((5, hq, hd))
+    q[..., 0], q[..., 40] = big, 1.0
+    q = q.view(5, hq * hd).to(BF)
+    keys, values = (x.flatten(0, 1)[:, 0] for x in O.decoded(pool))
+    table = torch.arange(94 * 5, dtype=torch.int32).view(5, 94).cuda()
+    lens = torch.full((5,), n, dtype=torch.int32, device="cuda")
+    for t in (table, _widened(table, 16)):
+        out = paged.paged_decode_q4(q.cuda(), pool.cuda(), t, lens, hq, scale).cpu().double().view(5, hq, hd)
+        for row in range(5):
+            kk, vv = keys[94 * 16 * row:][:n], values[94 * 16 * row:][:n]
+            s = (kk @ q[row, :hd].double()) * scale
+            p = torch.softmax(s, 0)
+            off = 2.0 ** -21 * (1 + (s.max() - s).clamp(max=1e6) / 0.693)
+            step = vv.abs().unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(-2) / 7
+            want = p @ vv
+            tol = 1.1 * (2.0 ** -11 * 15 * (p @ step) + 2 * ((p * off) @ vv.abs()) + 2.0 ** -8 * want.abs()) + 1e-30
+            assert bool(((out[row] - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -110, 2.0 ** 116, 2.0 ** 120, 2.0 ** 125])
+@pytest.mark.parametrize("hq", [2, 8])
+def test_attention_with_queries_at_the_ends_of_their_type(hq, size):
+    pool, table, lens = O.cache([77, 300], 1, 128, 16, BF, seed=2, device="cuda")
+    q = torch.randn((2, hq * 128), generator=torch.Generator().manual_seed(1)).clamp(-3.5, 3.5)
+    q = (q.double() * size).to(BF)
+    assert bool(torch.isfinite(q).all())
+    _check(q.cuda(), pool, table, lens, hq, 0.09 / size if size > 1 else 1e37)
