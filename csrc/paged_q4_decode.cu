@@ -236,8 +236,8 @@ __device__ __forceinline__ float2 q4_from(const float2& x, int half) {         /
 // long as the largest score is below kQ4Large. From there on a maximum rounded to fp32 would lie too far from the score it is
 // to be subtracted from (by 32 at 2^30: p of 2^32 or 2^-32), so `at` is the largest dot product, whose distance to others is
 // exact enough, and `off` stays small: both are in shared memory, and kQ4Far for an `off` sends every pass there. That such
-// scores may come costs others little (512 rows of 768 tokens 29.0 -> 29.2 us, 78 of 264 11.9 -> 12.5); the difference to `at` in
-// every pass instead took 30.3 us.
+// scores may come costs others little (512 rows of 768 tokens 29.0 -> 29.2 us, 78 of 264 11.9 -> 12.5); subtracting `at` in every
+// pass took 3 % more for the 512 rows.
 template <int NG>
 struct Q4State {
   float o[NG][2][4];            // V^T P^T: elements 32 g + 4 r + 2 m + (reg >> 1), columns 2c + (reg & 1); odd elements times

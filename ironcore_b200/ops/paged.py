@@ -307,7 +307,8 @@ def paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs=No
             continue
         k, v = (x.view(-1, hkv, hd).repeat_interleave(hq // hkv, 1)
                 for x in kv_read_q4_reference(pool, page * bs + tok % bs))
-        p = torch.softmax(torch.einsum("hd,nhd->hn", q[i].view(hq, hd).float(), k) * scale, dim=-1)
+        # 64 bits: products of a query, a key and the scale pass the range of 32
+        p = torch.softmax(torch.einsum("hd,nhd->hn", q[i].view(hq, hd).double(), k.double()) * scale, dim=-1).float()
         out[i] = torch.einsum("hn,nhd->hd", p, v).reshape(-1).to(q.dtype)
     return out
 

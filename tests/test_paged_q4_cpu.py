@@ -385,3 +385,13 @@ def test_prompts_of_any_type(family, dtype):
     got, lp2 = eng.generate(prompts.to(dtype), 5, temperature=0.0)
     assert set(seen) == {torch.int64}
     assert torch.equal(got, want) and torch.equal(lp, lp2)
+
+
+@pytest.mark.parametrize("scale,size", [(1e31, 1.0), (-1e31, 1.0), (1e38, 1.0), (-1e38, 1.0), (1e38, 2.0 ** 120), (1e-42, 2.0 ** 125)])
+def test_attention_restatement_at_the_ends(scale, size):
+    """Scores beyond what fp32 holds: the largest takes all, equal ones share."""
+    pool, table, lens = O.cache([30, 1, 17], 1, 64, 16, torch.float32)
+    q = torch.randn((3, 2 * 64), generator=torch.Generator().manual_seed(2)) * size
+    out = paged.paged_decode_q4(q, pool, table, lens, 2, scale)
+    want, _ = O.attention(q, *O.decoded(pool), table, lens, 2, scale)
+    assert torch.allclose(out.double(), want, atol=1e-5)
