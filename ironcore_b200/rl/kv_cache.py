@@ -204,6 +204,11 @@ class BlockKVCache(PagedCache):
     def bytes_per_token(self) -> int:
         return 2 * self.num_layers * self.kv_heads * self.head_dim * torch.empty((), dtype=self.dtype).element_size()
 
+    def on_kernels(self, dtype: torch.dtype) -> bool:
+        """Whether appending and attending run on kernels alone for rows of this type; the PyTorch restatements read lengths and
+        slots on the host, which no CUDA graph can capture."""
+        return dtype in (torch.bfloat16, torch.float16) and self.head_dim in (64, 128)
+
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
         paged.kv_append(k, v, self.k[layer], self.v[layer], slots)
 
@@ -228,6 +233,10 @@ class QuantizedKVCache(PagedCache):
 
     def bytes_per_token(self) -> int:
         return self.num_layers * self.kv_heads * self.head_dim * 9 // 8
+
+    def on_kernels(self, dtype: torch.dtype) -> bool:
+        """As of :class:`BlockKVCache`."""
+        return dtype in (torch.bfloat16, torch.float16)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
         paged.kv_append_q4(k, v, self.layers[layer], slots)

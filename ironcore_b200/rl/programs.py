@@ -48,6 +48,7 @@ class TransformerProgram:
             self.cache = QuantizedKVCache(*sizes, device=first.device)
         else:
             self.cache = BlockKVCache(*sizes, first.dtype, first.device)
+        self.capturable = self.cache.on_kernels(first.dtype)
 
     def refresh(self):
         pass
@@ -162,6 +163,7 @@ class StreamProgram:
     asked otherwise: a latent row is narrow, and its decode kernel copies a page with one box per 64 columns."""
 
     PAGE = 64
+    capturable = True
 
     def __init__(self, model, config, max_seqs: int, max_seq_len: int, block_size: Optional[int],
                  num_blocks: Optional[int]):

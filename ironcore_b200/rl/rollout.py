@@ -4,7 +4,8 @@ One step (:meth:`RolloutEngine.step`) runs the tokens it is given, for any set o
 lengths as one packed batch, one more token for each of several running requests, or any mixture. Requests own a cache
 sequence from their first token until they are ended. A decode step over ``n`` requests runs on static buffers and is
 captured in a CUDA graph the second time a batch of that size comes by (launch-bound regime: dozens of small kernels
-per layer). :meth:`RolloutEngine.generate` is the sampling loop on top.
+per layer); models whose cache has no kernels for their type or head size run every step as it is.
+:meth:`RolloutEngine.generate` is the sampling loop on top.
 (The reference only has a cache-less sampler that re-runs the whole prefix for every token:
 examples/generate_text.py:12-46.)
 """
@@ -50,7 +51,7 @@ class RolloutEngine:
         self.cache = self.program.cache
         self.max_seqs = max_seqs
         on_gpu = self.device.type == "cuda"
-        self.use_graph = on_gpu if use_cuda_graph is None else (use_cuda_graph and on_gpu)
+        self.use_graph = on_gpu and self.program.capturable and (use_cuda_graph is None or bool(use_cuda_graph))
         self._graphs: "OrderedDict[int, _DecodeGraph]" = OrderedDict()
         self._requests: Dict[Hashable, int] = {}
 

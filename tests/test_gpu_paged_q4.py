@@ -655,3 +655,29 @@ def test_attention_with_queries_at_the_ends_of_their_type(hq, size):
     q = (q.double() * size).to(BF)
     assert bool(torch.isfinite(q).all())
     _check(q.cuda(), pool, table, lens, hq, 0.09 / size if size > 1 else 1e37)
+
+
+@pytest.mark.parametrize("graph", [None, True])
+@pytest.mark.parametrize("bits,precision,head_dim", [(4, "fp32", 64), (16, "fp32", 64), (4, "bf16", 256), (16, "bf16", 256)])
+def test_rollouts_without_kernels_for_the_cache(bits, precision, head_dim, graph):
+    """Types and head sizes for which the cache's operators are PyTorch's run eagerly, whatever is asked for; the others captured."""
+    from ironcore_b200.config import validate_config
+    from ironcore_b200.models import LanguageModel
+    from ironcore_b200.parallel import mesh
+    from ironcore_b200.rl import RolloutEngine
+
+    mesh.destroy_model_parallel()
+    cfg = tiny_config("qwen", d_model=256, d_ffn=512, num_layers=2, num_attention_heads=4, num_attention_groups=2, head_dim=head_dim,
+                      max_seq_len=64, max_position_embeddings=64, precision=precision, vocab_size=512, qkv_bias=True)
+    cfg.trainer.use_flash_attn = False
+    cfg.rl.kv_cache_bits = bits
+    validate_config(cfg)
+    torch.manual_seed(3)
+    model = LanguageModel(cfg, device=torch.device("cuda")).cuda().eval()
+    eng = RolloutEngine(model, cfg, max_seqs=4, max_seq_len=64, use_cuda_graph=graph)
+    prompts = torch.randint(0, 512, (2, 19), generator=torch.Generator().manual_seed(1))
+    tokens, logps = eng.generate(prompts, 8, temperature=0.0, samples=2)
+    assert eng.use_graph == (bits == 4 and precision == "bf16")
+    assert any(g.graph is not None for g in eng._graphs.values()) == eng.use_graph
+    full = model.token_logprobs(tokens[:, :-1], tokens[:, 1:])[:, 18:]
+    assert bool(torch.isfinite(logps).all()) and (full - logps).abs().max().item() < (0.5 if bits == 4 else 0.15)

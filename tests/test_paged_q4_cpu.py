@@ -395,3 +395,19 @@ def test_attention_restatement_at_the_ends(scale, size):
     out = paged.paged_decode_q4(q, pool, table, lens, 2, scale)
     want, _ = O.attention(q, *O.decoded(pool), table, lens, 2, scale)
     assert torch.allclose(out.double(), want, atol=1e-5)
+
+
+def test_which_decode_steps_a_graph_can_hold():
+    """The restatements of the cache's operators read lengths on the host."""
+    from ironcore_b200.rl import BlockKVCache, QuantizedKVCache, RolloutEngine
+
+    sizes = dict(num_blocks=2, block_size=16, max_seqs=1, max_seq_len=32, device="cpu")
+    for hd, dtype, plain, four in ((64, torch.bfloat16, True, True), (128, torch.float16, True, True), (256, torch.bfloat16, False, True),
+                                   (64, torch.float32, False, False), (192, torch.float16, False, True)):
+        assert BlockKVCache(1, 1, hd, dtype=dtype, **sizes).on_kernels(dtype) == plain
+        assert QuantizedKVCache(1, 1, hd, **sizes).on_kernels(dtype) == four
+    for bits in (16, 4):
+        for kw in ({}, {"precision": "bf16"}):
+            cfg, model = _model(head_dim=64, num_attention_heads=4, **kw)
+            cfg.rl.kv_cache_bits = bits
+            assert RolloutEngine(model, cfg, max_seqs=2, max_seq_len=64).program.capturable == bool(kw)
