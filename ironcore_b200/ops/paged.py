@@ -367,7 +367,7 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
                     scale: Optional[float] = None, *, seqs: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, hq * hd] (row view, any pitch): row i against the first ``seq_lens[i]`` tokens of the sequence whose pages are
-    row ``seqs[i]`` of ``block_table`` (int32; None: row i) -> [T, hq * hd], into ``out`` (rows of any pitch) if given.
+    row ``seqs[i]`` of ``block_table`` (int32; None: row i) -> [T, hq * hd], into ``out`` (rows of any pitch, apart) if given.
     A row without tokens gives zeros. Page numbers outside the pool and table rows outside the table hold no tokens. A NaN
     among the keys or values of a sequence makes the heads that read it NaN. ``scale``: up to 1e38 of either sign."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
@@ -386,8 +386,9 @@ def paged_decode_q4(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tens
     table_rows, pages = block_table.shape
     if seqs is None and table_rows < t:
         raise ValueError(f"{t} rows for {table_rows} rows of pages")
-    if out is not None and (out.shape != shape or out.dtype != dtype or out.stride(1) != 1):
-        raise ValueError("out must have q's shape and type and neighbouring elements")
+    if out is not None and (out.shape != shape or out.dtype != dtype or out.stride(1) != 1
+                            or (t > 1 and out.stride(0) < shape[1])):
+        raise ValueError("out must have q's shape and type, neighbouring elements and rows that do not overlap")
     dev = pool.get_device()
     if not q.get_device() == block_table.get_device() == seq_lens.get_device() == dev \
             or (seqs is not None and seqs.get_device() != dev) or (out is not None and out.get_device() != dev):

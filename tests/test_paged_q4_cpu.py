@@ -411,3 +411,15 @@ def test_which_decode_steps_a_graph_can_hold():
             cfg, model = _model(head_dim=64, num_attention_heads=4, **kw)
             cfg.rl.kv_cache_bits = bits
             assert RolloutEngine(model, cfg, max_seqs=2, max_seq_len=64).program.capturable == bool(kw)
+
+
+def test_outputs_that_overlap_are_refused():
+    pool, table, lens = O.cache([7, 20], 1, 64, 16, torch.float32)
+    q = torch.randn((2, 128), generator=torch.Generator().manual_seed(1))
+    room = torch.zeros(400)
+    for stride in (0, 1, 127):
+        with pytest.raises(ValueError):
+            paged.paged_decode_q4(q, pool, table, lens, 2, out=room.as_strided((2, 128), (stride, 1)))
+    for n, stride in ((2, 128), (2, 131), (1, 0)):          # a single row has nothing to overlap
+        got = paged.paged_decode_q4(q[:n], pool, table[:n], lens[:n], 2, out=room.as_strided((n, 128), (stride, 1)))
+        assert torch.equal(got, paged.paged_decode_q4(q[:n], pool, table[:n], lens[:n], 2))
