@@ -315,8 +315,8 @@ def paged_decode_q4_reference(q, pool, block_table, seq_lens, hq, scale, seqs=No
 
 def kv_append_q4(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantise k, v [T, hkv * hd] (row views with arbitrary pitch) and write them to the cache rows ``slots`` (int64 [T],
-    block * block_size + offset; rows with a slot outside the pool are left out). Two rows with one slot: either may win,
-    element by element."""
+    block * block_size + offset; rows with a slot outside the pool are left out). No two rows may have one slot: what it holds
+    then is a mixture of both, codes and scales. Other slots are as they should be."""
     blocks, hkv, tiles, hd = _q4_sizes(pool)
     shape, dtype = k.shape, k.dtype
     if len(shape) != 2 or shape != v.shape or shape[1] != hkv * hd or dtype != v.dtype:

@@ -681,3 +681,39 @@ def test_rollouts_without_kernels_for_the_cache(bits, precision, head_dim, graph
     assert any(g.graph is not None for g in eng._graphs.values()) == eng.use_graph
     full = model.token_logprobs(tokens[:, :-1], tokens[:, 1:])[:, 18:]
     assert bool(torch.isfinite(logps).all()) and (full - logps).abs().max().item() < (0.5 if bits == 4 else 0.15)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_forked_captured_rollouts_follow_the_model(bits):
+    """Log-probs of samples that share their prompt's pages and run in captured steps, against the model without a cache. Sampled,
+    so that the forks differ; long enough for pages of their own."""
+    _, graph = _engine(bits, use_cuda_graph=True)
+    model = graph.model
+    prompts = torch.randint(0, 1024, (2, 37), generator=torch.Generator().manual_seed(1))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for _ in range(2):                                      # the second time on graphs from the first step on
+        tokens, logps = graph.generate(prompts, 40, temperature=1.0, samples=3, generator=g)
+        assert any(x.graph is not None for x in graph._graphs.values())
+        full = model.token_logprobs(tokens[:, :-1], tokens[:, 1:])[:, 36:]
+        assert bool(torch.isfinite(logps).all()) and (full - logps).abs().max().item() < (0.5 if bits == 4 else 0.15)
+        assert len({tuple(t) for t in tokens[:, 37:].tolist()}) == 6
+    assert graph.cache.free_blocks == graph.cache.num_blocks
+
+
+@pytest.mark.parametrize("t,hkv,hd", [(64, 2, 128), (4096, 8, 128)])
+def test_append_to_a_row_twice(t, hkv, hd):
+    """Rows of a call that share a slot leave something finite there and every other row of the pool as it should be."""
+    from ironcore_b200.ops import paged
+
+    k, v = _rows(t, hkv, hd, BF, seed=4)
+    slots = torch.arange(t)
+    for a in range(0, t, 50):
+        slots[a + 7] = a + 3                                # breaks up tiles, and shares a slot of one
+    shared = torch.zeros(t, dtype=torch.bool)
+    shared[torch.arange(0, t, 50) + 3] = True
+    want = torch.zeros(paged.q4_pool_shape(t // 16, hkv, 16, hd), dtype=torch.uint8)
+    got = want.cuda()
+    paged.kv_append_q4_reference(k.cpu(), v.cpu(), want, slots)
+    paged.kv_append_q4(k, v, got, slots.cuda())
+    for x, y in zip(paged.kv_read_q4(got, torch.arange(t).cuda(), BF), paged.kv_read_q4_reference(want, torch.arange(t), BF)):
+        assert torch.equal(x.cpu()[~shared], y[~shared]) and bool(torch.isfinite(x).all())
