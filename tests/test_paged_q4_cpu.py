@@ -423,3 +423,39 @@ def test_outputs_that_overlap_are_refused():
     for n, stride in ((2, 128), (2, 131), (1, 0)):          # a single row has nothing to overlap
         got = paged.paged_decode_q4(q[:n], pool, table[:n], lens[:n], 2, out=room.as_strided((n, 128), (stride, 1)))
         assert torch.equal(got, paged.paged_decode_q4(q[:n], pool, table[:n], lens[:n], 2))
+
+
+def _tp_rollout_worker(rank, world, out_path):
+    from ironcore_b200.config import validate_config
+    from ironcore_b200.models import LanguageModel
+    from ironcore_b200.parallel import mesh
+    from ironcore_b200.rl import RolloutEngine
+
+    cfg = tiny_config("llama", max_seq_len=64, max_position_embeddings=64, head_dim=64, num_attention_heads=4)
+    cfg.trainer.use_flash_attn = False
+    cfg.trainer(tensor_model_parallel_size=world)
+    cfg.parallel(world_size=world, rank=rank)
+    cfg.rl.kv_cache_bits = 4
+    validate_config(cfg)
+    mesh.initialize_model_parallel(world)
+    model = LanguageModel(cfg).eval()
+    eng = RolloutEngine(model, cfg, max_seqs=6, max_seq_len=64, block_size=16)
+    assert eng.cache.kv_heads == 2 // world
+    prompts = torch.randint(0, 512, (2, 21), generator=torch.Generator().manual_seed(4))
+    got = eng.generate(prompts, 12, temperature=0.0, samples=3)
+    assert eng.cache.free_blocks == eng.cache.num_blocks
+    if rank == 0:
+        torch.save(got, out_path)
+
+
+def test_rollouts_on_two_tensor_parallel_ranks_match_one(tmp_path):
+    """Each rank holds its kv heads in 4 bits, groups being within heads: the same codes, forks and tokens as on one rank."""
+    from helpers import run_distributed
+    from ironcore_b200.parallel import mesh
+
+    mesh.destroy_model_parallel()
+    a, b = str(tmp_path / "one.pt"), str(tmp_path / "two.pt")
+    run_distributed(_tp_rollout_worker, 1, a)
+    run_distributed(_tp_rollout_worker, 2, b)
+    (t1, lp1), (t2, lp2) = torch.load(a), torch.load(b)
+    assert torch.equal(t1, t2) and torch.allclose(lp1, lp2, atol=1e-4)
