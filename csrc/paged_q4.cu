@@ -12,8 +12,8 @@
 // Two forms of each direction: one thread per 8 elements of a row, for few rows; and four warps per tile of 16 rows and head, in
 // the order of the tile's lanes, so that all 18 hd bytes of the tile leave or arrive in 512-byte pieces (a row by itself touches
 // all of a tile's value sectors, two bytes in each). Rows that do not fill a tile go one by one. 32768 rows of 8 heads of 128:
-// append 41 us, 0.64 of the copy bandwidth, held by instruction issue (0.68 of the slots: eleven instructions an element, half of
-// them conversion and rounding); read 32 us, 0.83, held by its writes. One warp per tile took 61 and 39 us.
+// append 41 us from a cold cache, 0.64 of the copy bandwidth, held by instruction issue (0.68 of the slots: eleven instructions an
+// element, half of them conversion and rounding); read 32 us, 0.83, held by its writes. One warp per tile took 61 and 39 us.
 #include <string.h>
 
 #include "host_common.h"
@@ -559,9 +559,13 @@ kv_read_q4_tile_kernel(const uint8_t* __restrict__ pool, const long long* __rest
   }
 }
 
-// Elements of the keys from which on the kernels by tiles take a call. Below, a call is a decode step, whose rows lie in a tile
-// each, or too short for either kind to fill the GPU. In order, append by rows / by tiles: 8 heads of 128, 512 rows 7.4 / 9.4
-// us, 2048 rows 12.3 / 10.2, 8192 rows 31 / 21, 32768 rows 104 / 51; 1 head of 256, 8192 rows 12.3 / 14.4, 32768 rows 29 / 19.
+// Elements of the keys from which on the kernels by tiles take a call. What pays depends on the slots, which are on the device: rows
+// in order gain by tiles, rows that lie in a tile each (a decode step) lose. By rows / by tiles, us, from graphs: append, 8 heads of
+// 128, in order, 512 rows 3.1 / 2.2, 2048 rows (the threshold) 7.8 / 3.7, 8192 rows 27 / 12, 32768 rows 100 / 34; scattered,
+// 512 rows 3.1 / 5.1, 2048 rows 8.6 / 10.6, 8192 rows 27 / 35; 1 head of 256, 8192 rows (the threshold) in order 7.1 / 3.9,
+// scattered 7.9 / 12.9. Read, 8 heads of 128, in order, 2048 rows 6.3 / 3.1, scattered 7.4 / 7.4; 1 head of 256, 8192 rows 5.6
+// / 3.1 and 6.3 / 6.2. So the threshold lies above the decode steps but for the largest: 512 sequences of 32 heads of 128 are
+// on it, 10.7 us instead of 8.6.
 constexpr long long kQ4TileElements = 1LL << 21;
 
 // Heads that a block goes through one after the other, so that its look at the slots serves them all; blocks stay enough for 32

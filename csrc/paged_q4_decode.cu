@@ -17,7 +17,8 @@
 //     2^-24 of the head's largest.
 //   * p_t sv_tg is rounded to fp16 too. Its range is held by the maximum that the softmax subtracts: it runs over
 //     log2 p_t + log2 max_g |sv_tg| instead of log2 p_t, so that the largest product is 2^12 to 2^15, whatever the values'
-//     magnitude. Relative error 2^-11 down to 2^-26 of the largest contribution; sums, maxima and p itself stay in fp32.
+//     magnitude. Relative error 2^-11 down to 2^-26 of the largest contribution of any group of the head (a token whose values in
+//     one group are 2^20 times those elsewhere costs the other groups bits); sums, maxima and p itself stay in fp32.
 //   * Scores may have any size: from 2^22 on a maximum in fp32 does not do, and dot products are compared instead (Q4State).
 // Tokens outside the sequence get probability and value scale zero by selection, so nothing stale in a page (NaN scales
 // included) reaches a result. A page number outside the pool counts as a page outside the sequence.
@@ -30,8 +31,9 @@
 // and 21 matrix instructions (0.28 of their pipe). With 128 registers a thread, 16 warps on an SM issue 0.57 of the slots: the
 // kernels are held by the latencies of dependent instructions, not by memory. Captured calls over caches larger than L2, beside
 // the attention over the 16-bit cache: 512 rows of 768 tokens, 12 heads on 2 of 128, 28.8 us, 0.60 of the copy bandwidth (16 bits:
-// 109 us); 64 rows of 2000, 32 on 32, 100 us, 0.90 (388); 4 rows of 100000, 32 on 8, 84.8 us, 0.83 (385); 33 rows of up to 1500,
-// 12 on 12 of 64, 11.1 us (40); one row of 333, 5.2 us (9.6).
+// 109 us); 64 rows of 2000, 32 on 32, 103 us, 0.88 (391); 4 rows of 100000, 32 on 8, 86.6 us, 0.81 (381); 33 rows of up to 1500,
+// 12 on 12 of 64, 11.2 us (40); one row of 333, 5.5 us (9.6). Heads of 192 and 256 need up to 255 registers a thread: eight warps on
+// an SM hide the same latencies (64 rows of 4000, 8 on 1 of 256, 28.1 us, 0.40; of 192, 23.7, 0.36; of 1000 and 256, 13.6, 0.21).
 #include <math.h>
 #include <string.h>
 
@@ -44,8 +46,9 @@ namespace icb {
 
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = kQ4Warps * 32;
-// Least tiles of a warp: with fewer, joining the parts of a long row among short ones takes longer than what it gains. One row of
-// 8000 tokens among 255 of 100 (12 heads on 2): 42 us with 2, 23.5 with 6; 4 rows of 4000 (32 on 8): 14.6, 14.3, with 12 15.1.
+// Least tiles of a warp: with fewer, joining the parts of a long row among short ones takes longer than what it gains. With 2, 6 and
+// 12, us: one row of 8000 tokens among 255 of 100 (12 heads on 2, a table of 20000: in a table of 8000 it does not come here) 43.8,
+// 24.9, 24.7; 4 rows of 4000 (32 on 8) 15.8, 15.4, 16.2; 16 of 8000 (12 on 2) 20.7, 20.7, 21.0.
 constexpr int kQ4MinTiles = 6;
 constexpr int kQ4Whole = 8;                     // units of at most so many tiles are not divided among warps
 constexpr float kQ4Top = 12.f;                  // log2 of the largest fp16 probability times scale right after a new maximum
@@ -983,9 +986,12 @@ static int q4_blocks() {
 // ten warps to an SM, no more than two tiles each need, and so many that none has more than 32 tiles, for a long row among
 // short ones is its block's alone. Ranges cost some 10 us more, of which a part of a few tiles is too much to wait for them where
 // the units are few: what a warp has here beyond an even share of all tiles may be ten tiles of 128 elements a head. With
-// 128-element heads, this kernel and ranges, us: 512 rows of 768 tokens on 2 kv heads 28.8, 37.8; of 1536 46.8, 58.7; 8 of 4000 on
-// 32 30.4, 35.6; 64 of 8000 on 2 33.3, 43.7; 8 of 4000 on 8 16.8, 19.2; but 4 of 4000 on 8 16.3, 14.6; 16 of 8000 on 2 31.7, 20.5;
-// 4 of 30000 on 8 91, 35.7; 48 of up to 10000 on 8 39.7, 37.1. 64 rows of 4000 on 1 of 256: 36.8, 28.0.
+// 128-element heads, this kernel and ranges, us: 512 rows of 768 tokens on 2 kv heads 28.4, 38.7; of 1536 46.3, 59.3; 8 of 4000 on
+// 32 30.9, 35.5; 64 of 8000 on 2 33.3, 44.0; 8 of 4000 on 8 17.9, 19.8; but 4 of 4000 on 8 17.6, 15.4; 16 of 8000 on 2 32.4, 20.7;
+// 4 of 30000 on 8 92.2, 35.8; 48 of up to 10000 on 8 67.8, 65.2. 64 rows of 4000 on 1 of 256: 37.2, 28.1.
+// The rule knows the table's width and not the lengths, which are on the device: in tables much wider than their rows most warps of
+// a block have nothing. 512 rows of 100 tokens on 2 kv heads: 10.0 us in a table of 112 tokens, 10.2 in 1024, 12.9 in 2048, 19.5 in
+// 4096, 32 in 8192; of 768 tokens 28.7 in 768, 28.1 in 1536, 53 in 8192; one row of 8000 among 255 of 100 32.1 (24.9 by ranges).
 static int q4_unit_warps(int hd, long long units, long long tiles) {
   const int most = hd <= 128 ? 16 : 8;
   int warps = 1;

@@ -213,7 +213,7 @@ class RolloutEngine:
 
         ``prompts`` [S, P]: returns (tokens [S, P + N] including the prompt, log-probs of the N sampled tokens
         [S, N]). A list of token lists may be unequal, with one ``max_new_tokens`` or one per prompt and an optional
-        ``stop_token``; it runs in waves of up to ``max_seqs`` prompts whose requests leave the batch as they finish,
+        ``stop_token``; it runs in waves of up to ``max_seqs // samples`` prompts whose requests leave the batch as they finish,
         and returns (list of sampled tokens, list of their log-probs). ``samples`` continuations of every prompt,
         neighbours in the result ([S * samples, ...]): the prompt runs once and its cache is forked."""
         if samples < 1 or samples > self.max_seqs:
